@@ -251,6 +251,70 @@ int lb_rglru_gates_fwd(const void* gx, const void* ga, const void* x, const floa
 int lb_rglru_gates_bwd(const void* gx, const void* ga, const void* x, const float* sp, const void* da, const void* db,
                        void* dgx, void* dga, void* dx, float* dsp, long long rows, int C, void* stream);
 
+// Paged KV cache (paged_cache.cu, paged_attention.cu). Pools k_pages / v_pages: [n_pages, page, Hkv, D] bf16 given by
+// element strides (sp page, st token, sh head; channels contiguous, every stride a multiple of 8). table: int32
+// [n_seqs, cols] (row pitch table_stride), page of positions [i page, (i + 1) page) of a sequence. kv_len: int32 [n_seqs],
+// keys of a sequence, the new tokens included. cu_q: int32 [n_seqs + 1], first packed row of every sequence's new tokens,
+// or NULL for one token per sequence (T == n_seqs). The new tokens are the last positions of their sequence. Rows
+// that belong to no sequence, and positions below zero, are padding: zeros come out and nothing is written to the cache.
+// A page outside [0, n_pages) or a position past the table is recorded in the status word and skipped.
+typedef struct LbPagedAppendArgs {
+  const void *q, *k, *v;  // [T, H | Hkv | Hkv, D] bf16
+  void* q_out;            // [T, H, D] contiguous: q rotated (copied when cs is NULL)
+  void *k_pages, *v_pages;
+  const int* table;
+  const int* kv_len;
+  const int* cu_q;
+  const float* cs;  // [cs_rows, D / 2, 2] (cos, sin), or NULL: keys are stored as they are
+  uint32_t* status;
+  int T, n_seqs, H, Hkv, D, page, n_pages, cols, cs_rows;
+  long long table_stride;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  long long kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh;
+} LbPagedAppendArgs;
+int lb_paged_append(const LbPagedAppendArgs* a, void* stream);
+
+// pool[r, dst[i]] = pool[r, src[i]] for r < rows, i < n (int32 on the device); strides in bytes, multiples of 16.
+// No destination may repeat or be a source as well.
+int lb_copy_pages(void* pool, long long row_stride, long long page_stride, long long page_bytes, int rows, int n_pages,
+                  const int* src, const int* dst, int n, uint32_t* status, void* stream);
+
+// o[t, h] = softmax(scale q k^T) v over the visible keys: j <= p and (window <= 0 or j > p - window or j < sinks).
+typedef struct LbPagedAttnArgs {
+  const void* q;  // [T, H, D] bf16
+  const void *k_pages, *v_pages;
+  void* o;  // [T, H, D] contiguous
+  const int* table;
+  const int* kv_len;
+  const int* cu_q;
+  uint32_t* status;
+  int T, n_seqs, H, Hkv, D, page, n_pages, cols, window, sinks;
+  float scale;
+  long long table_stride;
+  long long q_st, q_sh;
+  long long kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh;
+} LbPagedAttnArgs;
+int lb_paged_attention(const LbPagedAttnArgs* a, void* stream);
+
+// Penalties, bias and mask on logits [N, V] (logits.cu). history: int64 [N, L], the first history_len[n] entries count
+// (ids outside [0, V) are ignored); those from prompt_len[n] on were generated (NULL: all). repetition / presence /
+// frequency: fp32 [N], or NULL and the scalar. bias: fp32, row pitch bias_stride (0: one row for all), or NULL. allowed:
+// bit mask, 32 tokens a word, row pitch allowed_stride words, or NULL. out may be logits.
+typedef struct LbPenalizeArgs {
+  const void* logits;
+  void* out;
+  const long long* history;
+  const int* history_len;
+  const int* prompt_len;
+  const float *repetition, *presence, *frequency;
+  const float* bias;
+  const uint32_t* allowed;
+  int N, V, L, dtype;
+  float repetition_s, presence_s, frequency_s;
+  long long ld_in, ld_out, history_stride, bias_stride, allowed_stride;
+} LbPenalizeArgs;
+int lb_penalize_logits(const LbPenalizeArgs* a, void* stream);
+
 // Number of kernels launched by this library in this process so far.
 long long lb_launch_count(void);
 void lb_launch_count_add(long long n);

@@ -70,6 +70,30 @@ class AttnArgs(C.Structure):
     ]
 
 
+class PagedAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_pages", "v_pages", "table", "kv_len", "cu_q", "cs",
+                                          "status")]
+    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "cs_rows")]
+    _fields_ += [(n, C.c_longlong) for n in ("table_stride", "q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "kp_sp",
+                                             "kp_st", "kp_sh", "vp_sp", "vp_st", "vp_sh")]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_pages", "v_pages", "o", "table", "kv_len", "cu_q", "status")]
+    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "window", "sinks")]
+    _fields_ += [("scale", C.c_float)]
+    _fields_ += [(n, C.c_longlong) for n in ("table_stride", "q_st", "q_sh", "kp_sp", "kp_st", "kp_sh", "vp_sp", "vp_st",
+                                             "vp_sh")]
+
+
+class PenalizeArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "out", "history", "history_len", "prompt_len", "repetition", "presence",
+                                          "frequency", "bias", "allowed")]
+    _fields_ += [(n, C.c_int) for n in ("N", "V", "L", "dtype")]
+    _fields_ += [(n, C.c_float) for n in ("repetition_s", "presence_s", "frequency_s")]
+    _fields_ += [(n, C.c_longlong) for n in ("ld_in", "ld_out", "history_stride", "bias_stride", "allowed_stride")]
+
+
 def lib_path() -> Path:
     return _LIB_PATH
 
@@ -138,6 +162,10 @@ def _declare(lib) -> None:
         "lb_scan_fwd": [vp, vp, ip, fp, vp, fp, fp, i, i, i, vp],
         "lb_scan_bwd": [vp, vp, vp, ip, fp, vp, vp, fp, i, i, i, vp],
         "lb_decode_attn": [vp, vp, vp, vp, vp, ip, ip, vp, i, i, i, i, ll, ll, f, vp],
+        "lb_paged_append": [C.POINTER(PagedAppendArgs), vp],
+        "lb_paged_attention": [C.POINTER(PagedAttnArgs), vp],
+        "lb_copy_pages": [vp, ll, ll, ll, i, i, ip, ip, i, vp, vp],
+        "lb_penalize_logits": [C.POINTER(PenalizeArgs), vp],
         "lb_conv1d_update": [vp, ll, vp, vp, vp, ll, i, i, i, i, vp],
         "lb_conv_states": [vp, ll, llp, llp, vp, i, i, i, vp],
         "lb_ssm_state_update": [fp, vp, ll, fp, fp, vp, ll, vp, ll, fp, i, vp, i, i, i, i, i, vp],

@@ -1,0 +1,107 @@
+"""Penalties, bias and grammar mask on the logits of a sampling step (``csrc/logits.cu``).
+
+Runs between the model and ``generation.sample_tokens`` (the step of apps/main/generate.py:49-63 that the reference takes
+on unmodified logits)."""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+from .paged import _launch, _refuse
+
+Knob = Optional[Union[float, torch.Tensor]]
+
+
+def _knob(value: Knob, name: str, N: int, neutral: float, dev):
+    """(per-row tensor or None, scalar) of a penalty given as a number, an fp32 [N] tensor or None."""
+    if value is None:
+        return None, neutral
+    if isinstance(value, torch.Tensor):
+        _refuse(value.shape != (N,) or value.dtype != torch.float32 or not value.is_contiguous() or value.device != dev,
+                f"{name} must be a number or a contiguous fp32 [N] tensor on the logits' device")
+        return value, neutral
+    return None, float(value)
+
+
+def penalize_logits_ref(logits, history, history_len, prompt_len=None, repetition=None, presence=None, frequency=None,
+                        bias=None, allowed=None):
+    N, V = logits.shape
+    x = logits.double() if logits.dtype == torch.float64 else logits.float()
+    at = torch.arange(history.shape[1], device=x.device).view(1, -1)
+    live = (at < history_len.view(N, 1)) & (history >= 0) & (history < V)
+    new = live if prompt_len is None else live & (at >= prompt_len.view(N, 1))
+    ids = history.clamp(0, V - 1)
+    seen = torch.zeros_like(x).scatter_add_(1, ids, live.to(x.dtype))
+    made = torch.zeros_like(x).scatter_add_(1, ids, new.to(x.dtype))
+    rep, pres, freq = (k.view(N, 1).to(x.dtype) if isinstance(k, torch.Tensor) else (neutral if k is None else float(k))
+                       for k, neutral in ((repetition, 1.0), (presence, 0.0), (frequency, 0.0)))
+    z = torch.where(seen > 0, torch.where(x > 0, x / rep, x * rep), x)
+    z = torch.where(made > 0, z - (pres + freq * made), z)
+    if bias is not None:
+        z = z + bias.to(x.dtype)
+    if allowed is not None:
+        tok = torch.arange(V, device=x.device)
+        z = z.masked_fill(((allowed[:, tok // 32] >> (tok % 32).int()) & 1) == 0, float("-inf"))
+    return z.to(logits.dtype)
+
+
+def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: torch.Tensor,
+                    prompt_len: Optional[torch.Tensor] = None, repetition: Knob = None, presence: Knob = None,
+                    frequency: Knob = None, bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Logits [N, V] (bf16 or fp32) after the penalties of each row's history, in their own dtype.
+
+    history       int64 [N, L] token ids, of which the first ``history_len[n]`` (int32) count; ids outside the vocabulary
+                  are ignored
+    prompt_len    int32 [N]: entries from here on were generated (None: all of them)
+    repetition    > 0; a token of the history has its logit divided by this if positive, else multiplied by it
+    presence      subtracted once from every generated token's logit
+    frequency     subtracted once per occurrence among the generated tokens
+    bias          fp32 [V] or [N, V], added
+    allowed       int32 [N, ceil(V / 32)]: bit (t % 32) of word t / 32 clear means token t becomes -inf, whatever its logit
+    out           destination, ``logits`` itself included; a new tensor by default
+
+    The penalties are numbers or fp32 [N] tensors. A row whose mask allows nothing comes out as -inf everywhere."""
+    _refuse(logits.dim() != 2, "logits must be [N, V]")
+    N, V = logits.shape
+    dev = logits.device
+    _refuse(history.dim() != 2 or history.shape[0] != N or history.dtype != torch.int64, "history must be int64 [N, L]")
+    for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):
+        _refuse(t is not None and (t.shape != (N,) or t.dtype != torch.int32), f"{name} must be int32 [N]")
+    rep_t, rep = _knob(repetition, "repetition", N, 1.0, dev)
+    _refuse(rep_t is None and not rep > 0.0, "repetition must be positive")
+    pres_t, pres = _knob(presence, "presence", N, 0.0, dev)
+    freq_t, freq = _knob(frequency, "frequency", N, 0.0, dev)
+    if bias is not None:
+        _refuse(bias.dtype != torch.float32 or bias.shape not in ((V,), (N, V)), "bias must be fp32 [V] or [N, V]")
+    if allowed is not None:
+        _refuse(allowed.dtype != torch.int32 or allowed.shape != (N, (V + 31) // 32), "allowed must be int32 [N, ceil(V / 32)]")
+    for t in (history, history_len, prompt_len, bias, allowed, out):
+        _refuse(t is not None and t.device != dev, "all tensors must be on one device")
+    if out is not None:
+        _refuse(out.shape != logits.shape or out.dtype != logits.dtype, "out must have the logits' shape and dtype")
+    _refuse(logits.requires_grad and torch.is_grad_enabled(), "penalize_logits has no gradient")
+    if not logits.is_cuda:
+        z = penalize_logits_ref(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, allowed)
+        return z if out is None else out.copy_(z)
+    _refuse(logits.dtype not in (torch.bfloat16, torch.float32), "the kernel takes bf16 and fp32 logits")
+    _refuse(N > 65535, "too many rows")
+    for t in (logits, history, history_len, prompt_len, bias, allowed, out):
+        _refuse(t is not None and t.shape[-1] > 1 and t.stride(-1) != 1, "rows must be contiguous")
+    if out is None:
+        out = torch.empty(N, V, dtype=logits.dtype, device=dev)
+    if N == 0 or V == 0:
+        return out
+    def p(t):
+        return None if t is None else t.data_ptr()
+
+    a = _lib.PenalizeArgs(
+        logits.data_ptr(), out.data_ptr(), history.data_ptr(), history_len.data_ptr(), p(prompt_len), p(rep_t), p(pres_t),
+        p(freq_t), p(bias), p(allowed), N, V, history.shape[1],
+        _lib.LB_BF16 if logits.dtype == torch.bfloat16 else _lib.LB_F32, rep, pres, freq,
+        logits.stride(0), out.stride(0), history.stride(0), 0 if bias is None or bias.dim() == 1 else bias.stride(0),
+        0 if allowed is None else allowed.stride(0))
+    _launch(_lib.load().lb_penalize_logits, a, dev, "lb_penalize_logits")
+    return out

@@ -1,0 +1,235 @@
+"""Paged-cache kernels against 64-bit forms (tests/paged_oracle.py says where the tolerances come from)."""
+import pytest
+import torch
+
+from lingua_b200.ops import _lib
+from lingua_b200.ops import paged as P
+from paged_oracle import append64, attention64, attention_tolerance, make_batch, rotary
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def attend(b, one=False, **kw):
+    return P.paged_attention(b["q"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"],
+                             cu_q=None if one else b["cu_q"], max_q=max(b["q_lens"] + [1]), **kw)
+
+
+def check(o, b, window=0, sinks=0, scale=None):
+    ref, mag = attention64(b, window, sinks, scale)
+    err = (o.double() - ref).abs()
+    assert torch.isfinite(o.float()).all()
+    bad = err > attention_tolerance(ref, mag)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, largest {err[bad].max():.3g} at {bad.nonzero()[0].tolist()}"
+
+
+MASKS = [(0, 0), (1, 0), (40, 0), (40, 5), (200, 33), (1000, 2)]
+
+
+@pytest.mark.parametrize("window,sinks", MASKS)
+@pytest.mark.parametrize("H,Hkv,D,page", [(1, 1, 128, 16), (8, 2, 128, 32), (6, 2, 64, 16), (16, 1, 128, 64), (4, 4, 64, 256),
+                                          (14, 2, 128, 128), (40, 2, 128, 16)])
+def test_one_token_per_sequence(H, Hkv, D, page, window, sinks):
+    kv = [1, 2, 0, 15, 16, 17, 63, 64, 65, 129, 300, 777]
+    b = make_batch([1] * len(kv), kv, H, Hkv, D, page, DEV, seed=H + page, release=(window, sinks) if window else None)
+    check(attend(b, one=True, window=window, sinks=sinks), b, window, sinks)
+    check(attend(b, window=window, sinks=sinks), b, window, sinks)  # the same through cu_q
+
+
+@pytest.mark.parametrize("window,sinks", MASKS)
+@pytest.mark.parametrize("H,Hkv,D,page", [(2, 2, 128, 16), (8, 2, 128, 64), (6, 2, 64, 32), (16, 1, 128, 128), (3, 1, 128, 256),
+                                          (7, 7, 64, 16), (48, 2, 128, 16)])
+def test_chunks(H, Hkv, D, page, window, sinks):
+    q = [1, 5, 0, 33, 130, 257, 1, 7]
+    kv = [1, 5, 40, 200, 130, 700, 321, 3]  # the last has more new tokens than keys: rows that see nothing
+    b = make_batch(q, kv, H, Hkv, D, page, DEV, seed=H + page, pad_rows=3, release=(window, sinks) if window else None)
+    o = attend(b, window=window, sinks=sinks)
+    check(o, b, window, sinks)
+    assert (o[-3:] == 0).all() and (o[sum(q) - 7:sum(q) - 4] == 0).all()
+
+
+@pytest.mark.parametrize("order", ["heads", "wide"])
+@pytest.mark.parametrize("q,kv", [([1, 1, 1], [40, 333, 65]), ([20, 150, 1], [40, 333, 65])])
+def test_memory_orders(order, q, kv):
+    b = make_batch(q, kv, 8, 2, 128, 32, DEV, order=order)
+    check(attend(b), b)
+
+
+@pytest.mark.parametrize("q,kv", [([1], [20001]), ([1, 1], [33000, 5]), ([300], [9000]), ([17, 1], [5000, 30])])
+def test_long_keys(q, kv):
+    b = make_batch(q, kv, 4, 1, 128, 64, DEV)
+    check(attend(b), b)
+
+
+def test_many_sequences():
+    kv = [(i * 37) % 150 for i in range(700)]
+    b = make_batch([1] * 700, kv, 2, 1, 128, 16, DEV)
+    check(attend(b, one=True), b)
+
+
+@pytest.mark.parametrize("scale", [0.0, 0.02, 1.0])
+def test_scale(scale):
+    for q, kv in (([1, 1], [100, 37]), ([140, 3], [300, 50])):
+        b = make_batch(q, kv, 8, 2, 128, 16, DEV, seed=3)
+        check(attend(b, scale=scale), b, scale=scale)
+
+
+def test_values_far_apart():
+    """A running maximum that grows late, and scores whose exponentials underflow."""
+    for q, kv in (([1], [700]), ([200], [700])):
+        b = make_batch(q, kv, 4, 4, 128, 16, DEV, seed=4)
+        k = b["k_pages"]
+        page = b["table"][0, 30].long()
+        k[page] = k[page] * 30
+        check(attend(b, scale=0.5), b, scale=0.5)
+
+
+def test_repeats_bit_for_bit_and_on_other_streams():
+    b = make_batch([1] * 5 + [300], [4000, 17, 900, 64, 2500, 2000], 8, 2, 128, 16, DEV)
+    first = attend(b)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for s in (s1, s2) * 4:  # calls that overlap
+        with torch.cuda.stream(s):
+            outs.append(attend(b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+
+
+@pytest.mark.parametrize("one", [True, False])
+def test_graph_replay_with_new_lengths(one):
+    q, kv = ([1, 1, 1], [500, 1, 900]) if one else ([30, 1, 200], [500, 1, 900])
+    b = make_batch(q, kv, 8, 2, 128, 16, DEV, poison=False)
+    cs = rotary(1000, 128, DEV)
+    attend(b, one)  # status word and kernels are loaded before the capture
+    P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"], b["cu_q"], cs)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            qr = P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"],
+                                None if one else b["cu_q"], cs)
+            o = attend({**b, "q": qr}, one)
+        graphs.append((g, qr, o))
+    for kv_new in ([300, 1, 640], [499, 0, 256]):
+        b["kv_len"].copy_(torch.tensor(kv_new, dtype=torch.int32))
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        now = {**b, "kv_lens": kv_new}
+        for _, qr, o in graphs:
+            check(o, {**now, "q": qr})
+
+
+@pytest.mark.parametrize("turn", [True, False])
+@pytest.mark.parametrize("H,Hkv,D,page", [(1, 1, 128, 16), (8, 2, 64, 32), (32, 8, 128, 64), (5, 5, 128, 256)])
+@pytest.mark.parametrize("order", ["pool", "heads", "wide"])
+def test_append(H, Hkv, D, page, order, turn):
+    q, kv = [3, 0, 20, 1, 1, 300, 4], [3, 9, 40, 0, 77, 301, 2]
+    b = make_batch(q, kv, H, Hkv, D, page, DEV, order=order, pad_rows=2, poison=order == "pool")
+    cs = rotary(400, D, DEV) if turn else None
+    kb, vb = b["k_pages"].clone(), b["v_pages"].clone()
+    raw = b["k"].clone()
+    out = P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"], b["cu_q"], cs)
+    ref, writes = append64(b, cs)
+    kw = kb.double()
+    for (pg, row), (k, v) in writes.items():
+        kw[pg, row], vb[pg, row] = k.to(DEV), v.to(DEV).bfloat16()
+    # a rotated value is one rounding to bf16 of two fp32 products: half a step, plus 2^-22 of the pair's size
+    pair = 8.0 * 2 ** -22 * 8
+    assert ((out.double().cpu() - ref).abs() <= ref.abs() * 2 ** -8 + pair).all()
+    same = torch.isnan(kw) | torch.isinf(kw) | ((b["k_pages"].double() - kw).abs() <= kw.abs() * 2 ** -8 + pair)
+    assert same.all()
+    assert torch.equal(torch.isnan(b["k_pages"]), torch.isnan(kw)) and torch.equal(torch.isinf(b["k_pages"]), torch.isinf(kw))
+    assert torch.equal(torch.nan_to_num(b["v_pages"].float()), torch.nan_to_num(vb.float()))
+    assert torch.equal(raw, b["k"])
+    if not turn:
+        assert torch.equal(out[:3], b["q"][:3])
+
+
+def test_append_one_token_and_same_bits_as_the_unpaged_rotation():
+    from lingua_b200.ops import functional as F
+
+    b = make_batch([1] * 4, [5, 90, 0, 33], 8, 2, 128, 16, DEV, poison=False)
+    cs = F.rope_table(128, 100, 10000.0, DEV)
+    q1 = P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"], cs=cs)
+    qkv = torch.cat((b["q"], b["k"]), dim=1).reshape(4, -1).contiguous()
+    F.rope_(qkv, cs, 10, 128, 4, torch.tensor([4, 89, 0, 32], dtype=torch.int32, device=DEV))
+    qkv = qkv.view(4, 10, 128)
+    live = [0, 1, 3]
+    assert torch.equal(q1[live], qkv[live, :8]) and (q1[2] == 0).all()
+    for s, p in ((0, 4), (1, 89), (3, 32)):
+        assert torch.equal(b["k_pages"][b["table"][s, p // 16].long(), p % 16], qkv[s, 8:])
+
+
+@pytest.mark.parametrize("dtype,page_shape", [(torch.bfloat16, (16, 2, 64)), (torch.float32, (4,)), (torch.uint8, (48,)),
+                                              (torch.bfloat16, (64, 16, 128)), (torch.bfloat16, (5, 3, 8))])
+@pytest.mark.parametrize("n", [1, 7, 40])
+def test_copy_pages(dtype, page_shape, n):
+    g = torch.Generator().manual_seed(n)
+    pool = torch.randint(0, 200, (3, 100, *page_shape), generator=g).to(dtype).to(DEV)
+    ids = torch.randperm(100, generator=g).int()
+    src, dst = ids[:n].clone(), ids[n:2 * n].clone()
+    src[-1] = src[0]  # a source may repeat
+    want = pool.clone()
+    want[:, dst.long().to(DEV)] = want[:, src.long().to(DEV)]
+    a = pool.clone()
+    assert P.copy_pages(a, src, dst) is a and torch.equal(a, want)
+    a = pool.clone()
+    assert torch.equal(P.copy_pages(a, src.to(DEV), dst.to(DEV)), want)
+    part = pool[1:, 0:100]  # rows of a larger pool
+    P.copy_pages(part, src, dst)
+    assert torch.equal(pool[1:], want[1:]) and not torch.equal(pool[0], want[0])
+
+
+def test_bad_pages_are_reported_not_followed():
+    """Ids outside the pool, positions past the table: skipped, recorded, everybody else served."""
+    b = make_batch([1, 1, 1], [40, 40, 40], 4, 2, 128, 16, DEV, poison=False)
+    b["table"][1, 1] = 10 ** 6
+    with pytest.raises(RuntimeError, match="status"):
+        o = attend(b, one=True)
+        _lib.check_status()
+    good = [0, 2]
+    ref, mag = attention64({**b, "table": b["table"].where(b["table"] < b["k_pages"].shape[0], 0)})
+    assert ((o.double() - ref).abs() <= attention_tolerance(ref, mag))[good].all() and torch.isfinite(o.float()).all()
+    b["q_lens"], many = [40, 40, 40], torch.randn(120, 4, 128, device=DEV).bfloat16()
+    b["cu_q"] = torch.tensor([0, 40, 80, 120], dtype=torch.int32, device=DEV)
+    b["q"] = many
+    with pytest.raises(RuntimeError, match="status"):
+        o = attend(b)
+        _lib.check_status()
+    assert torch.isfinite(o.float()).all()
+    with pytest.raises(RuntimeError, match="status"):
+        P.paged_append(many, many[:, :2], many[:, 2:], b["k_pages"], b["v_pages"], b["table"], b["kv_len"], b["cu_q"])
+        _lib.check_status()
+    with pytest.raises(RuntimeError, match="status"):
+        attend({**b, "kv_len": torch.full_like(b["kv_len"], 10 ** 9)})
+        _lib.check_status()
+    with pytest.raises(RuntimeError, match="status"):
+        P.copy_pages(b["k_pages"].unsqueeze(0), torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                     torch.tensor([10 ** 6, -1], dtype=torch.int32, device=DEV))
+        _lib.check_status()
+
+
+def test_refusals_on_the_gpu():
+    b = make_batch([1, 1], [20, 30], 4, 2, 128, 16, DEV, poison=False)
+    for kw in (dict(q=b["q"].half()), dict(k_pages=b["k_pages"].float(), v_pages=b["v_pages"].float(), q=b["q"].float()),
+               dict(table=b["table"].cpu()), dict(q=b["q"][..., ::2], k_pages=b["k_pages"][..., ::2], v_pages=b["v_pages"][..., ::2]),
+               dict(k_pages=b["k_pages"][:, :8], v_pages=b["v_pages"][:, :8]),
+               dict(q=b["q"][..., :32], k_pages=b["k_pages"][..., :32], v_pages=b["v_pages"][..., :32]),
+               dict(q=torch.zeros(2 * 4 * 128 + 1, device=DEV).bfloat16()[1:].view(2, 4, 128)),
+               dict(q=b["q"][:1].expand(2, 4, 128)),
+               dict(kv_len=torch.stack((b["kv_len"], b["kv_len"]), 1)[:, 0])):
+        with pytest.raises(ValueError):
+            attend({**b, **kw}, one=True)
+    for pool in (torch.zeros(1, 4, 3, device=DEV), torch.zeros(1, 4, 8, 8, device=DEV)[..., ::2],
+                 torch.zeros(1, 1, 8, device=DEV).expand(1, 4, 8)):
+        with pytest.raises(ValueError):
+            P.copy_pages(pool, torch.tensor([0], dtype=torch.int32), torch.tensor([1], dtype=torch.int32))
+    empty = make_batch([], [], 4, 2, 128, 16, DEV, poison=False)
+    assert attend(empty, one=True).shape == (0, 4, 128)
