@@ -294,7 +294,10 @@ typedef struct LbPagedAttnArgs {
   long long q_st, q_sh;
   long long kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh;
 } LbPagedAttnArgs;
-int lb_paged_attention(const LbPagedAttnArgs* a, void* stream);
+// page is a power of two >= 16. workspace: lb_paged_attention_workspace(a) bytes of device memory (16-byte aligned, contents
+// irrelevant, not shared with a call that may run at the same time), or NULL when that is 0.
+int lb_paged_attention(const LbPagedAttnArgs* a, void* workspace, void* stream);
+long long lb_paged_attention_workspace(const LbPagedAttnArgs* a);
 
 // Penalties, bias and mask on logits [N, V] (logits.cu). history: int64 [N, L], the first history_len[n] entries count
 // (ids outside [0, V) are ignored); those from prompt_len[n] on were generated (NULL: all). repetition / presence /

@@ -1,94 +1,500 @@
-// Attention of new tokens over a paged KV cache (see paged_cache.cu for the layout of cache and batch).
+// Attention of few new tokens per sequence over a paged KV cache (see paged_cache.cu for the layout of cache and batch).
 //
 // The query of a token at position p sees the keys j <= p of its sequence and, with a sliding window W, of those only
 // the ones with j > p - W or j < sinks. A row that sees no key (a padding row, an empty sequence) gives zeros.
 //
-// One block per (token, head): four warps stride over the keys with one online softmax each (running maximum m,
-// sum l, accumulator), joined in shared memory at the end.
+// Bound by reading every visible key and value row once (2 D 2 bytes per key and kv head; G = H / Hkv query heads share
+// them). Layout of the work:
+//  * An item is (sequence, kv head, 16 rows), the rows being (token, head of the group) pairs, so that one pass over the
+//    keys serves the whole group on m16n8k16 tensor-core products (16 x 8 keys of scores, then 16 rows x 8 channels).
+//  * The key axis of an item is cut into blocks of 64 keys. All blocks of all items, in order, are dealt out in equal
+//    contiguous shares to the blocks of a fixed grid, so a batch of any mix of lengths keeps every SM equally busy; an
+//    item that crosses a share boundary leaves partial results (running maximum, sum, unnormalised output, fp32) that
+//    a second small kernel joins. The shares follow from the lengths on the device: a captured graph can be replayed with
+//    other lengths. When the table's width allows no item longer than NOSPLIT_BLOCKS blocks, items are dealt out whole
+//    instead and the second kernel is not launched.
+//  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. A lane copies
+//    exactly the 16-byte pieces that it will feed to the tensor cores itself (the contraction index may be permuted
+//    freely if q and k agree, and so may the output channels), so the ring in shared memory needs no barrier:
+//    cp.async, wait for the own group, read back, multiply. Keys nobody may see are zero-filled instead of read, so what a
+//    page holds past the end of a sequence (or a page that was given back) never matters.
+#include <algorithm>
 #include "common.cuh"
 #include "lingua_b200.h"
 
 namespace lb {
 
+constexpr int DEC_BLOCK = 64;       // keys per block: 16 for each warp
+constexpr int DEC_ROWS = 16;
+constexpr int NOSPLIT_BLOCKS = 8;
+constexpr int MIN_SHARE = 2;
+constexpr float DEC_LOG2E = 1.4426950408889634f;
+
 template <int D>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const LbPagedAttnArgs a) {
-  constexpr int E = D / 32;  // channels of a lane
-  const int tok = blockIdx.x, h = blockIdx.y, hk = h / (a.H / a.Hkv);
+struct DecCfg {
+  static constexpr int KI = D / 32;                 // 16-byte pieces of one key row per lane
+  static constexpr int VG = D / 64;                 // 16-byte pieces of one value row per lane
+  static constexpr int PIECES = 2 * KI + 4 * VG;    // per lane and 16 keys: 2 key rows, 4 value rows
+  static constexpr int STAGE = PIECES * 512;        // bytes of one warp's stage
+  static constexpr int NST = D == 128 ? 3 : 6;
+  static constexpr int SMEM = 4 * NST * STAGE;      // 96 KB: two blocks per SM
+  static constexpr int OROW = D + 4;                // padded row of the merge buffer (floats)
+  static constexpr int SLOT = DEC_ROWS * D + 2 * DEC_ROWS;  // floats of one partial result
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;  // 0 bytes read: the destination is zero-filled
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// What a sequence asks for.
+struct DecSeq {
+  int q0, nq;       // its rows of q
+  long long pos0;   // position of its first new token (may be negative)
+  int end;          // visible keys end here
+  int wlo;          // first key inside some row's window
+  int sb, wb;       // 64-key blocks: [0, sb) for the first tokens, then from wb on
+  int nb;           // blocks of an item (at least one: rows that see nothing still get their zeros)
+  int rt;           // 16-row tiles
+};
+
+__device__ __forceinline__ DecSeq dec_seq(const LbPagedAttnArgs& a, int s, bool report) {
+  DecSeq r;
+  r.q0 = a.cu_q ? a.cu_q[s] : s;
+  r.nq = a.cu_q ? a.cu_q[s + 1] - r.q0 : 1;
+  const int cap = a.cols * a.page;
+  const int len = a.kv_len[s];
+  if (report && len > cap && a.status) atomicOr(a.status, ST_BAD_ARG | 0x43u);
+  if (r.q0 < 0 || r.nq < 0 || r.q0 > a.T - r.nq) {  // rows that q does not have
+    if (report && a.status) atomicOr(a.status, ST_BAD_ARG | 0x45u);
+    r.nq = 0;
+  }
+  r.pos0 = (long long)len - r.nq;
+  r.end = max(0, min(len, cap));
+  r.wlo = 0;
+  if (a.window > 0) r.wlo = (int)max(0ll, min((long long)r.end, r.pos0 - a.window + 1));
+  r.wb = r.wlo / DEC_BLOCK;
+  r.sb = min((min(a.sinks, r.wlo) + DEC_BLOCK - 1) / DEC_BLOCK, r.wb);
+  r.nb = max(1, r.sb + (r.end + DEC_BLOCK - 1) / DEC_BLOCK - r.wb);
+  const long long rows = (long long)r.nq * (a.H / a.Hkv);
+  r.rt = (int)((rows + DEC_ROWS - 1) / DEC_ROWS);
+  return r;
+}
+
+struct DecWork {  // found by one thread, read by the block
+  long long first, last;  // this block's share of the units [first, last)
+  int seq;                // sequence of `first`
+  long long offset;       // units of that sequence before `first`
+};
+
+// Workspace: per block two partial results (its first item when an earlier block began it, its last item when a later
+// block ends it) and one int4 header naming the item it began without ending: (sequence, kv head, row tile, parts).
+template <int D>
+__global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnArgs a, float* ws, int4* hdr) {
+  using Cfg = DecCfg<D>;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ long long warp_sum[4];
+  __shared__ DecWork work;
+  __shared__ float sm_m[4][DEC_ROWS], sm_l[4][DEC_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int seq = tok, n_new = 1, at = 0;
+  const int r = lane >> 2, c = lane & 3;
+  const int G = a.H / a.Hkv;
+  const bool split = ws != nullptr;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this block's share: a unit is one 64-key block of an item (or a whole item without splitting)
+  const int per = (a.n_seqs + 127) / 128;
+  const int s_lo = min(a.n_seqs, (int)threadIdx.x * per), s_hi = min(a.n_seqs, s_lo + per);
+  long long mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) {
+    const DecSeq q = dec_seq(a, s, blockIdx.x == 0);
+    mine += (long long)a.Hkv * q.rt * (split ? q.nb : 1);
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  before += incl - mine;
+  // no share is empty (the join kernel counts on that), and small problems are not cut finer than MIN_SHARE
+  const long long n_blocks = max(1ll, min((long long)gridDim.x, split ? total / MIN_SHARE : total));
+  const bool busy = blockIdx.x < n_blocks;
+  const long long u0 = busy ? total * blockIdx.x / n_blocks : 0, u1 = busy ? total * (blockIdx.x + 1) / n_blocks : 0;
+  if (u0 < u1 && u0 >= before && u0 < before + mine) {
+    long long at = before;
+    for (int s = s_lo; s < s_hi; ++s) {
+      const DecSeq q = dec_seq(a, s, false);
+      const long long n = (long long)a.Hkv * q.rt * (split ? q.nb : 1);
+      if (u0 < at + n) { work.first = u0; work.last = u1; work.seq = s; work.offset = u0 - at; break; }
+      at += n;
+    }
+  }
+  // rows of q that belong to no sequence
   if (a.cu_q) {
-    int lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_q[mid] <= tok) lo = mid; else hi = mid;
+    const int lo = a.n_seqs > 0 ? max(0, min(a.T, a.cu_q[0])) : 0;
+    const int hi = a.n_seqs > 0 ? max(lo, min(a.T, a.cu_q[a.n_seqs])) : 0;
+    const long long vec = (long long)a.H * D / 8;
+    for (int t = blockIdx.x; t < lo + a.T - hi; t += gridDim.x) {
+      uint4* row = reinterpret_cast<uint4*>((__nv_bfloat16*)a.o + (long long)(t < lo ? t : hi + t - lo) * a.H * D);
+      for (long long i = threadIdx.x; i < vec; i += 128) row[i] = make_uint4(0, 0, 0, 0);
     }
-    seq = lo;
-    n_new = a.cu_q[seq + 1] - a.cu_q[seq];
-    at = tok - a.cu_q[seq];
-    if (at < 0 || at >= n_new) seq = -1;
   }
-  long long n = 0;  // visible keys end here
-  if (seq >= 0) n = (long long)a.kv_len[seq] - n_new + at + 1;
-  if (n > (long long)a.cols * a.page) {
-    if (threadIdx.x == 0 && a.status) atomicOr(a.status, ST_BAD_ARG | 0x43u);
-    n = (long long)a.cols * a.page;
-  }
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
-  const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + tok * a.q_st + h * a.q_sh + lane * E;
+  if (split && threadIdx.x == 0) hdr[blockIdx.x] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  if (u0 >= u1) return;
+
+  const uint32_t ring = smem_u32(dyn) + warp * (Cfg::NST * Cfg::STAGE) + lane * 16;
+  const float sl2 = a.scale * DEC_LOG2E;
+  const int page_log = __ffs(a.page) - 1;
+  long long left = u1 - u0;
+  int seq = work.seq;
+  long long offset = work.offset;
+  for (; left > 0 && seq < a.n_seqs; ++seq, offset = 0) {
+    const DecSeq q = dec_seq(a, seq, false);
+    const int item_units = split ? q.nb : 1;
+    const long long n_items = (long long)a.Hkv * q.rt;
+    for (long long item = offset / item_units; left > 0 && item < n_items; ++item) {
+      const int hk = (int)(item / q.rt), rt = (int)(item % q.rt);
+      const int b0 = split ? (int)(offset - item * item_units > 0 ? offset - item * item_units : 0) : 0;
+      const int b1 = split ? (int)min((long long)q.nb, b0 + left) : q.nb;
+      left -= split ? b1 - b0 : 1;
+
+      // ---- q fragments: lane (r, c) holds channels 32 i + 8 c .. + 7 of rows r and r + 8
+      const int row0 = rt * DEC_ROWS;
+      const int n_rows = min(DEC_ROWS, q.nq * G - row0);
+      uint4 qf[Cfg::KI][2];
+      long long pos[2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) { q[e] = __bfloat162float(qp[e]) * a.scale; acc[e] = 0.f; }
-  const long long w0 = a.window > 0 ? n - a.window : 0;
-  for (long long j = warp; j < n; j += 4) {
-    if (j < w0 && j >= a.sinks) { j += (w0 - j) / 4 * 4; if (j < w0) continue; }
-    const int page = a.table[seq * a.table_stride + j / a.page];
-    if (page < 0 || page >= a.n_pages) {
-      if (lane == 0 && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
-      continue;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = row0 + r + 8 * hf;
+        const bool live = r + 8 * hf < n_rows;
+        pos[hf] = live ? q.pos0 + row / G : -1;
+        const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (long long)(q.q0 + row / G) * a.q_st +
+                                  (long long)(hk * G + row % G) * a.q_sh + 8 * c;
+#pragma unroll
+        for (int i = 0; i < Cfg::KI; ++i)
+          qf[i][hf] = live ? *reinterpret_cast<const uint4*>(qp + 32 * i) : make_uint4(0, 0, 0, 0);
+      }
+
+      // ---- pages of this warp's next 32 + 32 blocks, one per lane
+      const int* trow = a.table + (long long)seq * a.table_stride;
+      auto key_of = [&](int b) { return (b < q.sb ? b : b - q.sb + q.wb) * DEC_BLOCK + warp * 16; };
+      auto page_of = [&](int b) {
+        const int k = key_of(b);
+        return b < b1 && k < q.end ? __ldg(trow + (k >> page_log)) : -1;
+      };
+      int pg = page_of(b0 + lane), pg_next = -1;
+      auto issue = [&](int b) {
+        const int rel = b - b0;
+        if ((rel & 31) == 0 && rel) pg = pg_next;
+        if ((rel & 31) == 16) pg_next = page_of(b + 16 + lane);
+        const int page = __shfl_sync(0xFFFFFFFFu, pg, rel & 31);
+        const int kb = key_of(b);
+        const bool ok = page >= 0 && page < a.n_pages;
+        const int off = kb & (a.page - 1);
+        const long long pk = ok ? page * a.kp_sp + hk * a.kp_sh : 0, pv = ok ? page * a.vp_sp + hk * a.vp_sh : 0;
+        const uint32_t dst = ring + (rel % Cfg::NST) * Cfg::STAGE;
+        bool wanted = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int j = kb + t * 8 + r;
+          const bool vis = j < q.end && (j >= q.wlo || j < a.sinks);
+          wanted |= vis;
+          const __nv_bfloat16* p = (const __nv_bfloat16*)a.k_pages + pk + (ok && vis ? (off + t * 8 + r) * a.kp_st : 0) + 8 * c;
+#pragma unroll
+          for (int i = 0; i < Cfg::KI; ++i) cp_async16(dst + (t * Cfg::KI + i) * 512, p + 32 * i, ok && vis);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int jo = 2 * c + (t & 1) + (t >> 1) * 8, j = kb + jo;
+          const bool vis = j < q.end && (j >= q.wlo || j < a.sinks);
+          const __nv_bfloat16* p = (const __nv_bfloat16*)a.v_pages + pv + (ok && vis ? (off + jo) * a.vp_st : 0) + 8 * r;
+#pragma unroll
+          for (int g = 0; g < Cfg::VG; ++g) cp_async16(dst + (2 * Cfg::KI + t * Cfg::VG + g) * 512, p + 64 * g, ok && vis);
+        }
+        if (wanted && !ok && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
+      };
+
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float acc[Cfg::VG][8][4];
+#pragma unroll
+      for (int g = 0; g < Cfg::VG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[g][e][i] = 0.f;
+
+#pragma unroll
+      for (int st = 0; st < Cfg::NST - 1; ++st) {
+        if (b0 + st < b1) issue(b0 + st);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      for (int b = b0; b < b1; ++b) {
+        if (b + Cfg::NST - 1 < b1) issue(b + Cfg::NST - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::NST - 1) : "memory");
+        const uint32_t src = ring + ((b - b0) % Cfg::NST) * Cfg::STAGE;
+        float s[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+#pragma unroll
+          for (int i = 0; i < Cfg::KI; ++i) {
+            const uint4 k = lds128(src + (t * Cfg::KI + i) * 512);
+            mma16816(s[t], qf[i][0].x, qf[i][1].x, qf[i][0].y, qf[i][1].y, k.x, k.y);
+            mma16816(s[t], qf[i][0].z, qf[i][1].z, qf[i][0].w, qf[i][1].w, k.z, k.w);
+          }
+        }
+        // scores in units of log 2; s[t][2 hf + i]: row r + 8 hf, key kb + 8 t + 2 c + i
+        const int kb = key_of(b);
+        const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[t][x] *= sl2;
+            if (!whole) {
+              const int j = kb + 8 * t + 2 * c + (x & 1);
+              const long long p = pos[x >> 1];
+              if (j > p || j >= q.end || (a.window > 0 && j <= p - a.window && j >= a.sinks)) s[t][x] = -INFINITY;
+            }
+          }
+        // the running maximum only moves when it would be exceeded by more than 2^8 (probabilities stay below 2^8)
+        float mx[2];
+        bool grow = false;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
+          grow |= mx[hf] > m[hf] + 8.f;
+        }
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xFFFFFFFFu, mx[hf], 1));
+            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xFFFFFFFFu, mx[hf], 2));
+            if (mx[hf] > m[hf]) {
+              const float f = m[hf] == -INFINITY ? 0.f : exp2f(m[hf] - mx[hf]);
+              m[hf] = mx[hf];
+              l[hf] *= f;
+#pragma unroll
+              for (int g = 0; g < Cfg::VG; ++g)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { acc[g][e][2 * hf] *= f; acc[g][e][2 * hf + 1] *= f; }
+            }
+          }
+        }
+        // probabilities enter the second product in bf16 (half a step, 2^-8 of each); their sum is taken before that
+        uint32_t pa[2][2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float mm = m[hf] == -INFINITY ? 0.f : m[hf];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float p0 = exp2f(s[t][2 * hf] - mm), p1 = exp2f(s[t][2 * hf + 1] - mm);
+            l[hf] += p0 + p1;
+            pa[t][hf] = pack_bf16(p0, p1);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < Cfg::VG; ++g) {
+          uint32_t v[4][4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint4 u = lds128(src + (2 * Cfg::KI + t * Cfg::VG + g) * 512);
+            v[t][0] = u.x; v[t][1] = u.y; v[t][2] = u.z; v[t][3] = u.w;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+            mma16816(acc[g][e], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(v[0][e >> 1], v[1][e >> 1], sel),
+                     __byte_perm(v[2][e >> 1], v[3][e >> 1], sel));
+          }
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+      // ---- join the four warps
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        l[hf] += __shfl_xor_sync(0xFFFFFFFFu, l[hf], 1);
+        l[hf] += __shfl_xor_sync(0xFFFFFFFFu, l[hf], 2);
+        if (c == 0) { sm_m[warp][r + 8 * hf] = m[hf]; sm_l[warp][r + 8 * hf] = l[hf]; }
+      }
+      __syncthreads();
+      float* obuf = reinterpret_cast<float*>(dyn);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = r + 8 * hf;
+        if (row < n_rows) {
+          const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+          const float f = m[hf] == -INFINITY ? 0.f : exp2f(m[hf] - M);
+          float* dst = obuf + (warp * DEC_ROWS + row) * Cfg::OROW;
+#pragma unroll
+          for (int g = 0; g < Cfg::VG; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<float4*>(dst + 64 * g + 16 * c + 8 * i + e) =
+                    make_float4(acc[g][e][2 * hf + i] * f, acc[g][e + 1][2 * hf + i] * f, acc[g][e + 2][2 * hf + i] * f,
+                                acc[g][e + 3][2 * hf + i] * f);
+        }
+      }
+      __syncthreads();
+      const bool whole_item = b0 == 0 && b1 == q.nb;
+      float* slot = whole_item ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
+      for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
+        const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
+        const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(obuf + (w * DEC_ROWS + row) * Cfg::OROW + ch);
+          o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+          L += sm_m[w][row] == -INFINITY ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);
+        }
+        if (whole_item) {
+          const float inv = L > 0.f ? 1.f / L : 0.f;
+          const int gr = row0 + row;
+          __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
+          *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(slot + row * D + ch) = o;
+          if (ch == 0) { slot[DEC_ROWS * D + row] = M; slot[DEC_ROWS * D + DEC_ROWS + row] = L; }
+        }
+      }
+      if (!whole_item && b0 == 0 && threadIdx.x == 0) {
+        // units [u1 - (b1 - b0), + nb) hold this item: find the block its last unit belongs to
+        const long long end_unit = u1 - (b1 - b0) + q.nb - 1;
+        // share of unit u: the largest i with total * i / n_blocks <= u
+        long long i = (end_unit * n_blocks) / total;
+        while (i + 1 < n_blocks && total * (i + 1) / n_blocks <= end_unit) ++i;
+        while (i > 0 && total * i / n_blocks > end_unit) --i;
+        hdr[blockIdx.x] = make_int4(seq, hk, rt, (int)(i - blockIdx.x + 1));
+      }
+      __syncthreads();
     }
-    const __nv_bfloat16* kp = (const __nv_bfloat16*)a.k_pages + page * a.kp_sp + (j % a.page) * a.kp_st + hk * a.kp_sh + lane * E;
-    const __nv_bfloat16* vp = (const __nv_bfloat16*)a.v_pages + page * a.vp_sp + (j % a.page) * a.vp_st + hk * a.vp_sh + lane * E;
-    float s = 0.f;
+  }
+}
+
+// Joins the parts of the item that block `blockIdx.x` of the kernel above began and later blocks went on with: warps
+// take parts, lanes channels.
+template <int D>
+__global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAttnArgs a, const float* ws, const int4* hdr) {
+  using Cfg = DecCfg<D>;
+  constexpr int E = D / 32;
+  __shared__ float sm_o[8][D], sm_m[8], sm_l[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 h = hdr[blockIdx.x];
+  if (h.w == 0) return;
+  const DecSeq q = dec_seq(a, h.x, false);
+  const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = h.z * DEC_ROWS + blockIdx.y;
+  if (row >= q.nq * G) return;
+  auto slot = [&](int part) { return ws + (long long)(part == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + part)) * Cfg::SLOT; };
+  float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += q[e] * __bfloat162float(kp[e]);
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int part = warp; part < h.w; part += 8) {
+    const float* p = slot(part);
+    const float pm = p[DEC_ROWS * D + blockIdx.y], pl = p[DEC_ROWS * D + DEC_ROWS + blockIdx.y];
+    float x[E];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    const float mn = fmaxf(m, s), corr = __expf(m - mn), p = __expf(s - mn);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * corr + p * __bfloat162float(vp[e]);
-    l = l * corr + p;
+    for (int e = 0; e < E; ++e) x[e] = p[blockIdx.y * D + lane * E + e];
+    const float mn = fmaxf(m, pm);
+    const float fa = m == -INFINITY ? 0.f : exp2f(m - mn), fb = pm == -INFINITY ? 0.f : exp2f(pm - mn);
     m = mn;
-  }
-  __shared__ float sm_m[4], sm_l[4], sm_acc[4][D];
-  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+    l = l * fa + pl * fb;
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = acc[e];
+    for (int e = 0; e < E; ++e) o[e] = o[e] * fa + x[e] * fb;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
+  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
   __syncthreads();
   if (threadIdx.x < D) {
-    const float M = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    float L = 0.f, o = 0.f;
+    float M = -INFINITY, L = 0.f, x = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float c = sm_m[w] == -INFINITY ? 0.f : __expf(sm_m[w] - M);
-      L += sm_l[w] * c;
-      o += sm_acc[w][threadIdx.x] * c;
+    for (int w = 0; w < 8; ++w) M = fmaxf(M, sm_m[w]);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float f = sm_m[w] == -INFINITY ? 0.f : exp2f(sm_m[w] - M);
+      L += sm_l[w] * f;
+      x += sm_o[w][threadIdx.x] * f;
     }
-    ((__nv_bfloat16*)a.o)[((long long)tok * a.H + h) * D + threadIdx.x] = __float2bfloat16(L > 0.f ? o / L : 0.f);
+    ((__nv_bfloat16*)a.o)[((long long)(q.q0 + row / G) * a.H + h.y * G + row % G) * D + threadIdx.x] =
+        __float2bfloat16(L > 0.f ? x / L : 0.f);
   }
+}
+
+template <int D>
+static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
+  using Cfg = DecCfg<D>;
+  if (ensure_dyn_smem<paged_decode_kernel<D>>(Cfg::SMEM)) return 20;
+  const int grid = 2 * num_sms();
+  int4* hdr = ws ? reinterpret_cast<int4*>((float*)ws + 2ll * grid * Cfg::SLOT) : nullptr;
+  paged_decode_kernel<D><<<grid, 128, Cfg::SMEM, st>>>(a, (float*)ws, hdr);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (ws) {
+    // starts while the first kernel's last blocks run, and waits for all of it before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, a.cu_q ? DEC_ROWS : min(DEC_ROWS, a.H / a.Hkv));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D>, a, (const float*)ws, (const int4*)hdr) != cudaSuccess) {
+      return 400 + (int)cudaGetLastError();
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + (int)e;
 }
 
 }  // namespace lb
 
-extern "C" int lb_paged_attention(const LbPagedAttnArgs* a, void* stream) {
+extern "C" long long lb_paged_attention_workspace(const LbPagedAttnArgs* a) {
+  using namespace lb;
+  long long keys = (long long)a->cols * a->page;  // most keys a row can see
+  if (a->window > 0 && !a->cu_q) keys = std::min(keys, (long long)a->window + a->sinks);
+  if (keys <= NOSPLIT_BLOCKS * DEC_BLOCK) return 0;
+  const long long slot = a->D == 128 ? DecCfg<128>::SLOT : DecCfg<64>::SLOT;
+  return 2ll * num_sms() * (2 * slot * 4 + 16);
+}
+
+extern "C" int lb_paged_attention(const LbPagedAttnArgs* a, void* workspace, void* stream) {
   using namespace lb;
   if (a->D != 64 && a->D != 128) return 1;
-  if (a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->H > 65535) return 2;
+  if (a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv) return 2;
+  if (a->page < 16 || (a->page & (a->page - 1))) return 3;
+  if ((long long)a->cols * a->page > (1ll << 30)) return 4;
   if (a->T <= 0) return 0;
-  const dim3 grid(a->T, a->H);
-  if (a->D == 128)
-    paged_attn_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(*a);
-  else
-    paged_attn_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(*a);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : 400 + (int)e;
+  return a->D == 128 ? launch_decode<128>(*a, workspace, (cudaStream_t)stream)
+                     : launch_decode<64>(*a, workspace, (cudaStream_t)stream);
 }

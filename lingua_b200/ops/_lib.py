@@ -163,7 +163,7 @@ def _declare(lib) -> None:
         "lb_scan_bwd": [vp, vp, vp, ip, fp, vp, vp, fp, i, i, i, vp],
         "lb_decode_attn": [vp, vp, vp, vp, vp, ip, ip, vp, i, i, i, i, ll, ll, f, vp],
         "lb_paged_append": [C.POINTER(PagedAppendArgs), vp],
-        "lb_paged_attention": [C.POINTER(PagedAttnArgs), vp],
+        "lb_paged_attention": [C.POINTER(PagedAttnArgs), vp, vp],
         "lb_copy_pages": [vp, ll, ll, ll, i, i, ip, ip, i, vp, vp],
         "lb_penalize_logits": [C.POINTER(PenalizeArgs), vp],
         "lb_conv1d_update": [vp, ll, vp, vp, vp, ll, i, i, i, i, vp],
@@ -173,6 +173,9 @@ def _declare(lib) -> None:
         "lb_rglru_gates_fwd": [vp, vp, vp, fp, vp, vp, ll, i, vp],
         "lb_rglru_gates_bwd": [vp, vp, vp, fp, vp, vp, vp, vp, vp, fp, ll, i, vp],
     }
+    if hasattr(lib, "lb_paged_attention_workspace"):
+        lib.lb_paged_attention_workspace.argtypes = [C.POINTER(PagedAttnArgs)]
+        lib.lb_paged_attention_workspace.restype = C.c_longlong
     for name, args in sigs.items():
         if hasattr(lib, name):
             fn = getattr(lib, name)

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -76,13 +77,14 @@ def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
         _strided(v_pages, "v_pages")
 
 
+def _on(device: torch.device):
+    """Work on the operands' device, on that device's current stream, whichever device is current."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _launch(fn, args, device: torch.device, what: str) -> None:
-    """Launch on the operands' device, on that device's current stream."""
-    if device.index == torch.cuda.current_device():
+    with _on(device):
         rc = fn(C.byref(args), _lib.stream_ptr())
-    else:
-        with torch.cuda.device(device):
-            rc = fn(C.byref(args), _lib.stream_ptr())
     _lib.check(rc, what)
 
 
@@ -223,7 +225,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         None if cu_q is None else cu_q.data_ptr(), _status(q.device),
         T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, scale,
         block_table.stride(0), q.stride(0), q.stride(1), kp[0], kp[1], kp[2], vp[0], vp[1], vp[2])
-    _launch(_lib.load().lb_paged_attention, a, q.device, "lb_paged_attention")
+    lib = _lib.load()
+    with _on(q.device):
+        need = lib.lb_paged_attention_workspace(C.byref(a))
+        # a buffer of this call alone, from the allocator of the current stream (or graph)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        rc = lib.lb_paged_attention(C.byref(a), None if ws is None else ws.data_ptr(), _lib.stream_ptr())
+    _lib.check(rc, "lb_paged_attention")
     return out
 
 
@@ -261,7 +269,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
         src, dst = src.to(pool.device), dst.to(pool.device)
     _refuse(src.device != pool.device, "page ids must be on the pool's device or in host memory")
     src, dst = src.contiguous(), dst.contiguous()
-    with torch.cuda.device(pool.device):
+    with _on(pool.device):
         rc = _lib.load().lb_copy_pages(pool.data_ptr(), pool.stride(0) * es, pool.stride(1) * es, page_bytes, rows, n_pages,
                                        src.data_ptr(), dst.data_ptr(), n, _status(pool.device), _lib.stream_ptr())
     _lib.check(rc, "lb_copy_pages")
