@@ -13,11 +13,16 @@
 //    a second small kernel joins. The shares follow from the lengths on the device: a captured graph can be replayed with
 //    other lengths. When the table's width allows no item longer than NOSPLIT_BLOCKS blocks, items are dealt out whole
 //    instead and the second kernel is not launched.
-//  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. A lane copies
-//    exactly the 16-byte pieces that it will feed to the tensor cores itself (the contraction index may be permuted
-//    freely if q and k agree, and so may the output channels), so the ring in shared memory needs no barrier:
-//    cp.async, wait for the own group, read back, multiply. Keys nobody may see are zero-filled instead of read, so what a
-//    page holds past the end of a sequence (or a page that was given back) never matters.
+//  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. Every warp
+//    keeps its own ring of 16-key stages in shared memory, filled by TMA (boxes of 16 keys x 64 channels, 128-byte
+//    swizzle), so a stage is waited for and given back by one warp alone.
+//  * A lane reads 16-byte pieces and feeds them to the products as they are. That permutes the contraction index (the
+//    same way for q and k), the keys of an 8-key tile and the output channels; none of it changes a result. Column n of a
+//    tile is key sw(n) = (n >> 1) | (n & 1) << 2, and likewise lane row n takes the channel piece sw(n) of the values: with
+//    the swizzle, the eight lanes of a quarter warp then read eight different 16-byte columns of banks.
+//  * Keys that no row may see, and pages that are not there, never contribute: scores are replaced (not added to), and
+//    value pieces of hidden keys are zeroed in registers, so what a page holds past the end of a sequence (NaN included)
+//    or behind the window does not matter.
 #include <algorithm>
 #include "common.cuh"
 #include "lingua_b200.h"
@@ -32,20 +37,16 @@ constexpr float DEC_LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct DecCfg {
-  static constexpr int KI = D / 32;                 // 16-byte pieces of one key row per lane
-  static constexpr int VG = D / 64;                 // 16-byte pieces of one value row per lane
-  static constexpr int PIECES = 2 * KI + 4 * VG;    // per lane and 16 keys: 2 key rows, 4 value rows
-  static constexpr int STAGE = PIECES * 512;        // bytes of one warp's stage
+  static constexpr int KI = D / 32;            // 16-byte pieces of a key row that a lane takes
+  static constexpr int VG = D / 64;            // 64-channel boxes of a row
+  static constexpr int BOX = 16 * 128;         // 16 keys x 64 channels
+  static constexpr int STAGE = 2 * VG * BOX;   // bytes of one warp's stage: key boxes, then value boxes
   static constexpr int NST = D == 128 ? 3 : 6;
-  static constexpr int SMEM = 4 * NST * STAGE;      // 96 KB: two blocks per SM
+  static constexpr int SMEM = 4 * NST * STAGE + 1024;  // 97 KB: two blocks per SM
   static constexpr int OROW = D + 4;                // padded row of the merge buffer (floats)
   static constexpr int SLOT = DEC_ROWS * D + 2 * DEC_ROWS;  // floats of one partial result
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 16 : 0;  // 0 bytes read: the destination is zero-filled
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -53,7 +54,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -101,9 +102,13 @@ struct DecWork {  // found by one thread, read by the block
 // Workspace: per block two partial results (its first item when an earlier block began it, its last item when a later
 // block ends it) and one int4 header naming the item it began without ending: (sequence, kv head, row tile, parts).
 template <int D>
-__global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnArgs a, float* ws, int4* hdr) {
+__global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_constant__ CUtensorMap tk,
+                                                              const __grid_constant__ CUtensorMap tv,
+                                                              const LbPagedAttnArgs a, float* ws, int4* hdr) {
   using Cfg = DecCfg<D>;
-  extern __shared__ __align__(16) uint8_t dyn[];
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t full[4][Cfg::NST];
+  __shared__ int abort_flag;
   __shared__ long long warp_sum[4];
   __shared__ DecWork work;
   __shared__ float sm_m[4][DEC_ROWS], sm_l[4][DEC_ROWS];
@@ -111,6 +116,15 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
   const int r = lane >> 2, c = lane & 3;
   const int G = a.H / a.Hkv;
   const bool split = ws != nullptr;
+  const uint32_t dyn0 = (smem_u32(dyn) + 1023u) & ~1023u;  // the swizzle pattern repeats every 1024 bytes
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int w = 0; w < 4; ++w)
+      for (int st = 0; st < Cfg::NST; ++st) mbar_init(smem_u32(&full[w][st]), 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this block's share: a unit is one 64-key block of an item (or a whole item without splitting)
@@ -163,7 +177,12 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
   __syncthreads();
   if (u0 >= u1) return;
 
-  const uint32_t ring = smem_u32(dyn) + warp * (Cfg::NST * Cfg::STAGE) + lane * 16;
+  const uint32_t ring = dyn0 + warp * (Cfg::NST * Cfg::STAGE);
+  const uint32_t bars = smem_u32(&full[warp][0]);
+  uint32_t parity = 0;  // bit st: phase the next wait on stage st completes
+  int head = 0;         // stage of the next block to be read
+  bool alive = true;
+  const int sr = (r >> 1) | ((r & 1) << 2);  // sw(r)
   const float sl2 = a.scale * DEC_LOG2E;
   const int page_log = __ffs(a.page) - 1;
   long long left = u1 - u0;
@@ -204,35 +223,26 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
         return b < b1 && k < q.end ? __ldg(trow + (k >> page_log)) : -1;
       };
       int pg = page_of(b0 + lane), pg_next = -1;
-      auto issue = [&](int b) {
+      auto issue = [&](int b, int st) {
         const int rel = b - b0;
         if ((rel & 31) == 0 && rel) pg = pg_next;
         if ((rel & 31) == 16) pg_next = page_of(b + 16 + lane);
-        const int page = __shfl_sync(0xFFFFFFFFu, pg, rel & 31);
-        const int kb = key_of(b);
-        const bool ok = page >= 0 && page < a.n_pages;
-        const int off = kb & (a.page - 1);
-        const long long pk = ok ? page * a.kp_sp + hk * a.kp_sh : 0, pv = ok ? page * a.vp_sp + hk * a.vp_sh : 0;
-        const uint32_t dst = ring + (rel % Cfg::NST) * Cfg::STAGE;
-        bool wanted = false;
+        int page = __shfl_sync(0xFFFFFFFFu, pg, rel & 31);
+        if (lane == 0) {
+          const int kb = key_of(b), off = kb & (a.page - 1);
+          if (page < 0 || page >= a.n_pages) {
+            // hidden keys need no page; a visible key without one is an error. Outside the pool TMA fills with zeros.
+            const bool seen = kb < q.end && (kb + 16 > q.wlo || kb < a.sinks);
+            if (seen && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
+            page = a.n_pages;
+          }
+          const uint32_t bar = bars + 8 * st, dst = ring + st * Cfg::STAGE;
+          mbar_arrive_expect_tx(bar, Cfg::STAGE);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int j = kb + t * 8 + r;
-          const bool vis = j < q.end && (j >= q.wlo || j < a.sinks);
-          wanted |= vis;
-          const __nv_bfloat16* p = (const __nv_bfloat16*)a.k_pages + pk + (ok && vis ? (off + t * 8 + r) * a.kp_st : 0) + 8 * c;
+          for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + g * Cfg::BOX, &tk, bar, 64 * g, off, hk, page);
 #pragma unroll
-          for (int i = 0; i < Cfg::KI; ++i) cp_async16(dst + (t * Cfg::KI + i) * 512, p + 32 * i, ok && vis);
+          for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + (Cfg::VG + g) * Cfg::BOX, &tv, bar, 64 * g, off, hk, page);
         }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int jo = 2 * c + (t & 1) + (t >> 1) * 8, j = kb + jo;
-          const bool vis = j < q.end && (j >= q.wlo || j < a.sinks);
-          const __nv_bfloat16* p = (const __nv_bfloat16*)a.v_pages + pv + (ok && vis ? (off + jo) * a.vp_st : 0) + 8 * r;
-#pragma unroll
-          for (int g = 0; g < Cfg::VG; ++g) cp_async16(dst + (2 * Cfg::KI + t * Cfg::VG + g) * 512, p + 64 * g, ok && vis);
-        }
-        if (wanted && !ok && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
       };
 
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -244,38 +254,54 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[g][e][i] = 0.f;
 
-#pragma unroll
-      for (int st = 0; st < Cfg::NST - 1; ++st) {
-        if (b0 + st < b1) issue(b0 + st);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+      auto next = [](int st) { return st + 1 == Cfg::NST ? 0 : st + 1; };
+      int fill = head;
+      for (int b = b0; b < min(b1, b0 + Cfg::NST); ++b) {
+        issue(b, fill);
+        fill = next(fill);
       }
-      for (int b = b0; b < b1; ++b) {
-        if (b + Cfg::NST - 1 < b1) issue(b + Cfg::NST - 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::NST - 1) : "memory");
-        const uint32_t src = ring + ((b - b0) % Cfg::NST) * Cfg::STAGE;
-        float s[2][4];
+      for (int b = b0; alive && b < b1; ++b) {
+        alive = mbar_wait(bars + 8 * head, (parity >> head) & 1, &abort_flag, a.status, 0x46);
+        alive = __all_sync(0xFFFFFFFFu, alive);
+        if (!alive) break;
+        parity ^= 1u << head;
+        const uint32_t kbox = ring + head * Cfg::STAGE, vbox = kbox + Cfg::VG * Cfg::BOX;
+        uint4 kf[2][Cfg::KI], vf[4][Cfg::VG];
+        // key sw(r) + 8 t: its row is row & 7 == sw(r) of the swizzle pattern, pieces 4 (i & 1) + c of box i >> 1
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < Cfg::KI; ++i)
+            kf[t][i] = lds128(kbox + (i >> 1) * Cfg::BOX + (sr + 8 * t) * 128 + (((4 * (i & 1) + c) ^ sr) << 4));
+        // keys c, c + 4, c + 8, c + 12; channel piece sw(r)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int g = 0; g < Cfg::VG; ++g)
+            vf[t][g] = lds128(vbox + g * Cfg::BOX + (c + 4 * t) * 128 + ((sr ^ ((c + 4 * t) & 7)) << 4));
+        // two accumulators for each 8 keys: chains of dependent products half as long
+        float s[2][4], s2[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+          for (int i = 0; i < 4; ++i) s[t][i] = s2[t][i] = 0.f;
 #pragma unroll
           for (int i = 0; i < Cfg::KI; ++i) {
-            const uint4 k = lds128(src + (t * Cfg::KI + i) * 512);
+            const uint4 k = kf[t][i];
             mma16816(s[t], qf[i][0].x, qf[i][1].x, qf[i][0].y, qf[i][1].y, k.x, k.y);
-            mma16816(s[t], qf[i][0].z, qf[i][1].z, qf[i][0].w, qf[i][1].w, k.z, k.w);
+            mma16816(s2[t], qf[i][0].z, qf[i][1].z, qf[i][0].w, qf[i][1].w, k.z, k.w);
           }
         }
-        // scores in units of log 2; s[t][2 hf + i]: row r + 8 hf, key kb + 8 t + 2 c + i
+        // scores in units of log 2; s[t][2 hf + i]: row r + 8 hf, key kb + 8 t + sw(2 c + i) = kb + 8 t + c + 4 i
         const int kb = key_of(b);
         const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            s[t][x] *= sl2;
+            s[t][x] = (s[t][x] + s2[t][x]) * sl2;
             if (!whole) {
-              const int j = kb + 8 * t + 2 * c + (x & 1);
+              const int j = kb + 8 * t + c + 4 * (x & 1);
               const long long p = pos[x >> 1];
               if (j > p || j >= q.end || (a.window > 0 && j <= p - a.window && j >= a.sinks)) s[t][x] = -INFINITY;
             }
@@ -316,14 +342,20 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
             pa[t][hf] = pack_bf16(p0, p1);
           }
         }
+        if (!whole) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int j = kb + c + 4 * t;
+            if (j >= q.end || (j < q.wlo && j >= a.sinks))
+#pragma unroll
+              for (int g = 0; g < Cfg::VG; ++g) vf[t][g] = make_uint4(0, 0, 0, 0);
+          }
+        }
 #pragma unroll
         for (int g = 0; g < Cfg::VG; ++g) {
           uint32_t v[4][4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint4 u = lds128(src + (2 * Cfg::KI + t * Cfg::VG + g) * 512);
-            v[t][0] = u.x; v[t][1] = u.y; v[t][2] = u.z; v[t][3] = u.w;
-          }
+          for (int t = 0; t < 4; ++t) { v[t][0] = vf[t][g].x; v[t][1] = vf[t][g].y; v[t][2] = vf[t][g].z; v[t][3] = vf[t][g].w; }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
@@ -331,8 +363,16 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
                      __byte_perm(v[2][e >> 1], v[3][e >> 1], sel));
           }
         }
+        // every lane's pieces are in registers (the products needed them): the stage can be filled again
+        __syncwarp();
+        if (b + Cfg::NST < b1) issue(b + Cfg::NST, head);
+        head = next(head);
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      // a wait ran out (recorded in the status word): copies in flight land before shared memory is given up
+      if (!alive) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
 
       // ---- join the four warps
 #pragma unroll
@@ -342,7 +382,8 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
         if (c == 0) { sm_m[warp][r + 8 * hf] = m[hf]; sm_l[warp][r + 8 * hf] = l[hf]; }
       }
       __syncthreads();
-      float* obuf = reinterpret_cast<float*>(dyn);
+      if (abort_flag) return;  // read by all after the same barrier
+      float* obuf = reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)));
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int row = r + 8 * hf;
@@ -356,7 +397,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int e = 0; e < 8; e += 4)
-                *reinterpret_cast<float4*>(dst + 64 * g + 16 * c + 8 * i + e) =
+                *reinterpret_cast<float4*>(dst + 64 * g + 32 * i + 8 * c + e) =  // pieces sw(2 c + i) = c + 4 i
                     make_float4(acc[g][e][2 * hf + i] * f, acc[g][e + 1][2 * hf + i] * f, acc[g][e + 2][2 * hf + i] * f,
                                 acc[g][e + 3][2 * hf + i] * f);
         }
@@ -394,6 +435,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const LbPagedAttnA
         while (i > 0 && total * i / n_blocks > end_unit) --i;
         hdr[blockIdx.x] = make_int4(seq, hk, rt, (int)(i - blockIdx.x + 1));
       }
+      fence_proxy_async_smem();  // the merge buffer becomes the ring again: ordinary accesses before TMA writes
       __syncthreads();
     }
   }
@@ -455,7 +497,11 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
   if (ensure_dyn_smem<paged_decode_kernel<D>>(Cfg::SMEM)) return 20;
   const int grid = 2 * num_sms();
   int4* hdr = ws ? reinterpret_cast<int4*>((float*)ws + 2ll * grid * Cfg::SLOT) : nullptr;
-  paged_decode_kernel<D><<<grid, 128, Cfg::SMEM, st>>>(a, (float*)ws, hdr);
+  // pools as (channel, row of the page, head, page), read in boxes of 64 channels x 16 rows
+  CUtensorMap tk, tv;
+  if (make_tmap_4d(&tk, a.k_pages, 2, D, a.page, a.kp_st, a.Hkv, a.kp_sh, a.n_pages, a.kp_sp, 64, 16)) return 10;
+  if (make_tmap_4d(&tv, a.v_pages, 2, D, a.page, a.vp_st, a.Hkv, a.vp_sh, a.n_pages, a.vp_sp, 64, 16)) return 11;
+  paged_decode_kernel<D><<<grid, 128, Cfg::SMEM, st>>>(tk, tv, a, (float*)ws, hdr);
   g_launches.fetch_add(1, std::memory_order_relaxed);
   if (ws) {
     // starts while the first kernel's last blocks run, and waits for all of it before it reads

@@ -67,7 +67,7 @@ def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
     _refuse(dt != torch.bfloat16, "the kernels take bf16")
     _refuse(D not in HEAD_DIMS, f"head dim must be one of {HEAD_DIMS}, got {D}")
     _refuse(k_pages.shape[1] not in PAGE_SIZES, f"page size must be one of {PAGE_SIZES}, got {k_pages.shape[1]}")
-    _refuse(H > 65535, "too many heads")
+    _refuse(k_pages.shape[0] < 1, "the pool has no pages")
     _refuse(not kv_len.is_contiguous() or (cu_q is not None and not cu_q.is_contiguous())
             or (block_table.shape[1] > 1 and block_table.stride(1) != 1), "kv_len, cu_q and table rows must be contiguous")
     _strided(q, "q")
