@@ -294,6 +294,26 @@ int make_tmap_4d(CUtensorMap* out, const void* base, int esz, long long inner, l
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
+// 4-D map with a box of any shape; strides of dims 1 to 3 in elements (ignored for an extent of 1).
+int make_tmap_box(CUtensorMap* out, const void* base, int esz, const long long (&dims)[4], const long long (&strides)[3],
+                  const int (&box)[4]) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return -1;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+  }
+  for (int i = 0; i < 3; ++i)
+    s[i] = dims[i + 1] > 1 ? (cuuint64_t)(strides[i] * esz) : i ? s[i - 1] : (cuuint64_t)(dims[0] * esz);
+  const CUtensorMapDataType dt = esz == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : esz == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return (int)enc(out, dt, 4, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 static int g_num_sms = 0;
 int num_sms() {
   if (!g_num_sms) {

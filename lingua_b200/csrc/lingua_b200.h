@@ -289,7 +289,8 @@ typedef struct LbPagedAttnArgs {
   const int* cu_q;
   uint32_t* status;
   int T, n_seqs, H, Hkv, D, page, n_pages, cols, window, sinks;
-  float scale;
+  int max_q;  // most new tokens of a sequence: chooses the kernel, nothing else
+  float scale;  // >= 0
   long long table_stride;
   long long q_st, q_sh;
   long long kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh;
@@ -334,6 +335,9 @@ struct LbGemmArgsFwd;
 int make_tmap_4d(CUtensorMap* out, const void* base, int esz, long long inner, long long outer,
                  long long ld, int nb0, long long bs0, int nb1, long long bs1, int box_inner,
                  int box_outer);
+// 4-D map with a box of any shape; strides of dims 1 to 3 in elements.
+int make_tmap_box(CUtensorMap* out, const void* base, int esz, const long long (&dims)[4], const long long (&strides)[3],
+                  const int (&box)[4]);
 // Opt a kernel in to `bytes` of dynamic shared memory. The attribute belongs to the (function, device) pair,
 // so it is set once per device that launches the kernel, with that device current. Returns 0 on success.
 template <auto Kern>
@@ -349,6 +353,9 @@ int ensure_dyn_smem(int bytes) {
 }
 // two-SM (cta_group::2) 256 x 256-tile variant, gemm2.cu
 int gemm2_dispatch(const LbGemmArgs& a, cudaStream_t s);
+// chunks of new tokens over a paged cache on tcgen05, paged_attention_chunk.cu
+int paged_chunk_dispatch(const LbPagedAttnArgs& a, void* ws, cudaStream_t s);
+long long paged_chunk_workspace(int D);
 int gemm2_fp8_dispatch(const LbGemmFp8Args& a, cudaStream_t s);
 }
 #endif

@@ -525,8 +525,19 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
 
 }  // namespace lb
 
+namespace lb {
+// Up to CHUNK_ROWS rows (new tokens x heads of a group) a sequence's keys pass through the few-token kernel once or twice;
+// beyond that the tcgen05 kernel, which needs one pass for 256 rows, is faster.
+constexpr int CHUNK_ROWS = 16;
+static bool use_chunk(const LbPagedAttnArgs& a) {
+  const int G = a.H / a.Hkv;
+  return a.cu_q && G <= 128 && (long long)a.max_q * G > CHUNK_ROWS;
+}
+}  // namespace lb
+
 extern "C" long long lb_paged_attention_workspace(const LbPagedAttnArgs* a) {
   using namespace lb;
+  if (use_chunk(*a)) return paged_chunk_workspace(a->D);
   long long keys = (long long)a->cols * a->page;  // most keys a row can see
   if (a->window > 0 && !a->cu_q) keys = std::min(keys, (long long)a->window + a->sinks);
   if (keys <= NOSPLIT_BLOCKS * DEC_BLOCK) return 0;
@@ -541,6 +552,7 @@ extern "C" int lb_paged_attention(const LbPagedAttnArgs* a, void* workspace, voi
   if (a->page < 16 || (a->page & (a->page - 1))) return 3;
   if ((long long)a->cols * a->page > (1ll << 30)) return 4;
   if (a->T <= 0) return 0;
+  if (use_chunk(*a)) return workspace ? paged_chunk_dispatch(*a, workspace, (cudaStream_t)stream) : 5;
   return a->D == 128 ? launch_decode<128>(*a, workspace, (cudaStream_t)stream)
                      : launch_decode<64>(*a, workspace, (cudaStream_t)stream);
 }

@@ -80,7 +80,8 @@ class PagedAppendArgs(C.Structure):
 
 class PagedAttnArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k_pages", "v_pages", "o", "table", "kv_len", "cu_q", "status")]
-    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "window", "sinks")]
+    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "window", "sinks",
+                                         "max_q")]
     _fields_ += [("scale", C.c_float)]
     _fields_ += [(n, C.c_longlong) for n in ("table_stride", "q_st", "q_sh", "kp_sp", "kp_st", "kp_sh", "vp_sp", "vp_st",
                                              "vp_sh")]

@@ -214,6 +214,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     T, H, D = q.shape
     n_pages, P, Hkv, _ = k_pages.shape
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    _refuse(not scale >= 0.0, "scale must not be negative")
     if not q.is_cuda:
         return paged_attention_ref(q, k_pages, v_pages, block_table, kv_len, cu_q, scale, window, sinks)
     out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
@@ -223,7 +224,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     a = _lib.PagedAttnArgs(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
         None if cu_q is None else cu_q.data_ptr(), _status(q.device),
-        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, scale,
+        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, max_q, scale,
         block_table.stride(0), q.stride(0), q.stride(1), kp[0], kp[1], kp[2], vp[0], vp[1], vp[2])
     lib = _lib.load()
     with _on(q.device):
