@@ -18,12 +18,17 @@
 //  * Keys past the end of a sequence and behind the window lie in the same pages as visible ones. Their scores are
 //    replaced by -inf, and their V rows are zeroed in shared memory by the softmax threads before P is handed over (0 x NaN
 //    would reach every row). Pages that are missing are requested outside the pool, which TMA fills with zeros.
+#include <type_traits>
 #include "common.cuh"
 #include "lingua_b200.h"
 
 namespace lb {
 
-constexpr int CK_THREADS = 320;  // TMA warp, MMA warp, two softmax warpgroups
+// Control warpgroup (a TMA warp, an MMA warp, two idle ones) and two softmax warpgroups. A softmax thread holds 128
+// scores: registers move from the control warps to it, within what the block was launched with (384 x 168 =
+// 128 x 88 + 256 x 208).
+constexpr int CK_THREADS = 384;
+constexpr int CK_REGS_CONTROL = 88, CK_REGS_SOFTMAX = 208;
 constexpr int CK_HALF = 128 * 128;  // 128 rows x 64 channels: one swizzled box of a tile
 constexpr float CK_LOG2E = 1.4426950408889634f;
 
@@ -91,13 +96,10 @@ struct CkWalk {
   long long left;            // key tiles still to do
 };
 
-template <int D>
-__device__ __forceinline__ uint64_t ck_desc_k(uint32_t tile, int k) {
-  return make_smem_desc(tile + (k >> 2) * CK_HALF + (k & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t ck_desc_mn(uint32_t tile, int k) {
-  return make_smem_desc(tile + k * 2048, CK_HALF, 1024);
-}
+// Descriptors of the k-th 16-deep slice of a tile: the start address (in units of 16 bytes, the low field) moves by
+// 32 bytes inside a 64-channel half of a K-major tile, by 16 rows of 128 bytes of an MN-major one.
+__device__ __forceinline__ uint64_t ck_slice_k(uint64_t tile, int k) { return tile + (((k >> 2) * CK_HALF + (k & 3) * 32) >> 4); }
+__device__ __forceinline__ uint64_t ck_slice_mn(uint64_t tile, int k) { return tile + (k * 2048 >> 4); }
 
 template <int D>
 __global__ void __launch_bounds__(CK_THREADS, 1)
@@ -283,123 +285,129 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, &abort_flag, a.status, site)) != 0;
   };
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA
-    uint32_t kv = 0, piece = 0;  // key tiles and pieces requested so far
-    const int page_log = __ffs(a.page) - 1;
-    const int rows = min(a.page, 128);  // rows of a box
-    const int n_box = 128 / rows;       // boxes of a key tile
-    const uint32_t q_bytes = NH * tpt * G * 128;
-    walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
-      const int* trow = a.table + (long long)w.seq * a.table_stride;
-      auto page_of = [&](int i) {  // page of box `lane` of the i-th key tile
-        const int key = ck_tile(t, i) * 128 + lane * rows;
-        int pg = a.n_pages;
-        if (lane < n_box && i < i1 && key < t.hi && (key + rows > t.lo || key < a.sinks)) {
-          pg = __ldg(trow + (key >> page_log));
-          if (pg < 0 || pg >= a.n_pages) {
-            if (a.status) atomicOr(a.status, ST_BAD_ARG | 0x54u);
-            pg = a.n_pages;
-          }
-        }
-        return pg;
-      };
-      int pg = page_of(i0);
-      if (!wait_all(q_empty, (piece & 1) ^ 1, 0x61)) return false;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (t.n_tok1 > 0 ? 2 : 1) * q_bytes);
-        for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
-          for (int h = 0; h < NH; ++h)
-            tma_load_4d(sQ(s) + h * CK_HALF, &tq, q_full, 64 * h, w.hk * G, q.q0 + t.tok0 + s * tpt, 0);
-      }
-      ++piece;
-      for (int i = i0; i < i1; ++i, ++kv) {
-        const int s = kv % NST;
-        const uint32_t ph = ((kv / NST) & 1) ^ 1;
-        const int off = (ck_tile(t, i) * 128 + lane * rows) & (a.page - 1);
-        const int next = page_of(i + 1);
-        if (!wait_all(k_empty(s), ph, 0x62)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(k_full(s), Cfg::TILE);
-        __syncwarp();
-        if (lane < n_box)
-          for (int h = 0; h < NH; ++h)
-            tma_load_4d(sK(s) + h * CK_HALF + lane * rows * 128, &tk, k_full(s), 64 * h, off, w.hk, pg);
-        if (!wait_all(v_empty(s), ph, 0x63)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(v_full(s), Cfg::TILE);
-        __syncwarp();
-        if (lane < n_box)
-          for (int h = 0; h < NH; ++h)
-            tma_load_4d(sV(s) + h * CK_HALF + lane * rows * 128, &tv, v_full(s), 64 * h, off, w.hk, pg);
-        pg = next;
-      }
-      return true;
-    });
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
-      uint32_t kv = 0, piece = 0, n_p[2] = {0, 0};
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_REGS_CONTROL));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA
+      uint32_t kv = 0, piece = 0;  // key tiles and pieces requested so far
+      const int page_log = __ffs(a.page) - 1;
+      const int rows = min(a.page, 128);  // rows of a box
+      const int n_box = 128 / rows;       // boxes of a key tile
+      const uint32_t q_bytes = NH * tpt * G * 128;
       walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
-        int last[2] = {-1, -1};  // last active key tile of each query tile
-        for (int s = 0; s < 2; ++s)
-          for (int i = i1 - 1; i >= i0 && last[s] < 0; --i)
-            if (ck_active(a, t, s, ck_tile(t, i))) last[s] = i;
-        bool begun[2] = {false, false};
-        // MMAs of one thread run in issue order: S_t(i + 1) overwrites P_t(i) only after O_t += P_t V(i) has read it, and
-        // a commit after S_t(i + 1) also covers that product.
-        auto issue_s = [&](int s, int st) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) umma_f16(tS(s), ck_desc_k<D>(sQ(s), k), ck_desc_k<D>(sK(st), k), IDESC_S, k != 0);
-          umma_commit(s_full(s));
-        };
-        auto issue_pv = [&](int s, int st, int i) -> bool {
-          if (!mbar_wait(p_full(s), n_p[s] & 1, &abort_flag, a.status, 0x64)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tO(s), tS(s) + k * 8, ck_desc_mn(sV(st), k), IDESC_O, (begun[s] || k != 0) ? 1u : 0u);
-          begun[s] = true;
-          ++n_p[s];
-          if (i == last[s]) umma_commit(o_done(s));
-          return true;
-        };
-        auto scores = [&](int i, int s, bool& ready) -> bool {  // S of query tile s for key tile i
-          const uint32_t n = kv + (i - i0);
-          const int st = n % NST;
-          if (!ready) {
-            if (!mbar_wait(k_full(st), (n / NST) & 1, &abort_flag, a.status, 0x65)) return false;
-            tc_fence_after();
-            ready = true;
+        const int* trow = a.table + (long long)w.seq * a.table_stride;
+        auto page_of = [&](int i) {  // page of box `lane` of the i-th key tile
+          const int key = ck_tile(t, i) * 128 + lane * rows;
+          int pg = a.n_pages;
+          if (lane < n_box && i < i1 && key < t.hi && (key + rows > t.lo || key < a.sinks)) {
+            pg = __ldg(trow + (key >> page_log));
+            if (pg < 0 || pg >= a.n_pages) {
+              if (a.status) atomicOr(a.status, ST_BAD_ARG | 0x54u);
+              pg = a.n_pages;
+            }
           }
-          if (ck_active(a, t, s, ck_tile(t, i))) issue_s(s, st);
-          if (s == 1) umma_commit(k_empty(st));
-          if (s == 1 && i + 1 == i1) umma_commit(q_empty);
-          return true;
+          return pg;
         };
-        if (!mbar_wait(q_full, piece & 1, &abort_flag, a.status, 0x66)) return false;
-        ++piece;
-        tc_fence_after();
-        bool ready = false;
-        if (!scores(i0, 0, ready) || !scores(i0, 1, ready)) return false;
-        for (int i = i0; i < i1; ++i) {
-          const uint32_t n = kv + (i - i0);
-          const int st = n % NST, kt = ck_tile(t, i);
-          const bool a0 = ck_active(a, t, 0, kt), a1 = ck_active(a, t, 1, kt);
-          ready = false;
-          if (!mbar_wait(v_full(st), (n / NST) & 1, &abort_flag, a.status, 0x67)) return false;
-          tc_fence_after();
-          if (a0 && !issue_pv(0, st, i)) return false;
-          if (i + 1 < i1 && !scores(i + 1, 0, ready)) return false;
-          if (a1 && !issue_pv(1, st, i)) return false;
-          umma_commit(v_empty(st));
-          if (i + 1 < i1 && !scores(i + 1, 1, ready)) return false;
+        int pg = page_of(i0);
+        if (!wait_all(q_empty, (piece & 1) ^ 1, 0x61)) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, (t.n_tok1 > 0 ? 2 : 1) * q_bytes);
+          for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
+            for (int h = 0; h < NH; ++h)
+              tma_load_4d(sQ(s) + h * CK_HALF, &tq, q_full, 64 * h, w.hk * G, q.q0 + t.tok0 + s * tpt, 0);
         }
-        kv += i1 - i0;
+        ++piece;
+        for (int i = i0; i < i1; ++i, ++kv) {
+          const int s = kv % NST;
+          const uint32_t ph = ((kv / NST) & 1) ^ 1;
+          const int off = (ck_tile(t, i) * 128 + lane * rows) & (a.page - 1);
+          const int next = page_of(i + 1);
+          if (!wait_all(k_empty(s), ph, 0x62)) return false;
+          if (lane == 0) mbar_arrive_expect_tx(k_full(s), Cfg::TILE);
+          __syncwarp();
+          if (lane < n_box)
+            for (int h = 0; h < NH; ++h)
+              tma_load_4d(sK(s) + h * CK_HALF + lane * rows * 128, &tk, k_full(s), 64 * h, off, w.hk, pg);
+          if (!wait_all(v_empty(s), ph, 0x63)) return false;
+          if (lane == 0) mbar_arrive_expect_tx(v_full(s), Cfg::TILE);
+          __syncwarp();
+          if (lane < n_box)
+            for (int h = 0; h < NH; ++h)
+              tma_load_4d(sV(s) + h * CK_HALF + lane * rows * 128, &tv, v_full(s), 64 * h, off, w.hk, pg);
+          pg = next;
+        }
         return true;
       });
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA
+      if (lane == 0) {
+        uint32_t kv = 0, piece = 0, n_p[2] = {0, 0};
+        walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
+          int last[2] = {-1, -1};  // last active key tile of each query tile
+          for (int s = 0; s < 2; ++s)
+            for (int i = i1 - 1; i >= i0 && last[s] < 0; --i)
+              if (ck_active(a, t, s, ck_tile(t, i))) last[s] = i;
+          bool begun[2] = {false, false};
+          // MMAs of one thread run in issue order: S_t(i + 1) overwrites P_t(i) only after O_t += P_t V(i) has read it, and
+          // a commit after S_t(i + 1) also covers that product.
+          auto issue_s = [&](int s, int st) {
+            const uint64_t dq = make_smem_desc(sQ(s), 16, 1024), dk = make_smem_desc(sK(st), 16, 1024);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) umma_f16(tS(s), ck_slice_k(dq, k), ck_slice_k(dk, k), IDESC_S, k != 0);
+            umma_commit(s_full(s));
+          };
+          auto issue_pv = [&](int s, int st, int i) -> bool {
+            if (!mbar_wait(p_full(s), n_p[s] & 1, &abort_flag, a.status, 0x64)) return false;
+            tc_fence_after();
+            const uint64_t dv = make_smem_desc(sV(st), CK_HALF, 1024);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_f16_ts(tO(s), tS(s) + k * 8, ck_slice_mn(dv, k), IDESC_O, (begun[s] || k != 0) ? 1u : 0u);
+            begun[s] = true;
+            ++n_p[s];
+            if (i == last[s]) umma_commit(o_done(s));
+            return true;
+          };
+          auto scores = [&](int i, int s, bool& ready) -> bool {  // S of query tile s for key tile i
+            const uint32_t n = kv + (i - i0);
+            const int st = n % NST;
+            if (!ready) {
+              if (!mbar_wait(k_full(st), (n / NST) & 1, &abort_flag, a.status, 0x65)) return false;
+              tc_fence_after();
+              ready = true;
+            }
+            if (ck_active(a, t, s, ck_tile(t, i))) issue_s(s, st);
+            if (s == 1) umma_commit(k_empty(st));
+            if (s == 1 && i + 1 == i1) umma_commit(q_empty);
+            return true;
+          };
+          if (!mbar_wait(q_full, piece & 1, &abort_flag, a.status, 0x66)) return false;
+          ++piece;
+          tc_fence_after();
+          bool ready = false;
+          if (!scores(i0, 0, ready) || !scores(i0, 1, ready)) return false;
+          for (int i = i0; i < i1; ++i) {
+            const uint32_t n = kv + (i - i0);
+            const int st = n % NST, kt = ck_tile(t, i);
+            const bool a0 = ck_active(a, t, 0, kt), a1 = ck_active(a, t, 1, kt);
+            ready = false;
+            if (!mbar_wait(v_full(st), (n / NST) & 1, &abort_flag, a.status, 0x67)) return false;
+            tc_fence_after();
+            if (a0 && !issue_pv(0, st, i)) return false;
+            if (i + 1 < i1 && !scores(i + 1, 0, ready)) return false;
+            if (a1 && !issue_pv(1, st, i)) return false;
+            umma_commit(v_empty(st));
+            if (i + 1 < i1 && !scores(i + 1, 1, ready)) return false;
+          }
+          kv += i1 - i0;
+          return true;
+        });
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    const int wt = (warp - 2) >> 2;  // query tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_REGS_SOFTMAX));
+    const int wt = (warp - 4) >> 2;  // query tile
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
@@ -429,13 +437,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         tmem_wait_ld();
         const bool masked = k0 + 128 > min(p_first + 1, q.end) || (a.window > 0 && k0 < lo_last && k0 + 128 > a.sinks);
         if (masked) {
+          // key k0 + x is visible for x < up, and x >= down or x < top; every other score becomes -inf
+          const int up = hi - k0;
+          if (a.window > 0) {
+            const int down = lo - k0, top = a.sinks - k0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int j = k0 + c * 32 + e;
-              if (j >= hi || (j < lo && j >= a.sinks)) sv[c][e] = 0xFF800000u;
-            }
+              for (int e = 0; e < 32; ++e) {
+                const int x = c * 32 + e;
+                sv[c][e] = ((x < up) & ((x >= down) | (x < top))) ? sv[c][e] : 0xFF800000u;
+              }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sv[c][e] = c * 32 + e < up ? sv[c][e] : 0xFF800000u;
+          }
         }
         float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -470,44 +488,43 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         // P = exp2(S scale - m) in bf16 (half a step, 2^-8 of each); the row sum is taken before that rounding. Two of
         // eight exponentials run on the FMA pipe, so that the MUFU is not the limit.
         const uint64_t sl2_2 = pack_f2(sl2, sl2), negm2 = pack_f2(-m_eff, -m_eff);
-        uint64_t ls2 = 0ull;
+        uint64_t ls2[2] = {0ull, 0ull};
+        auto exponentials = [&](auto poly) {  // one straight run of code per kind of tile: a branch in it would serialise it
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t pk[32];
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t pk[32];
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const int c = 2 * hf + cc;
+            for (int g = 0; g < 8; ++g) {
+              const uint32_t* s8 = &sv[2 * hf + (g >> 2)][8 * (g & 3)];
+              uint64_t x[4], p[4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              const uint64_t x01 = ffma2(pack_u2(sv[c][e], sv[c][e + 1]), sl2_2, negm2);
-              const uint64_t x23 = ffma2(pack_u2(sv[c][e + 2], sv[c][e + 3]), sl2_2, negm2);
-              const uint64_t x45 = ffma2(pack_u2(sv[c][e + 4], sv[c][e + 5]), sl2_2, negm2);
-              const uint64_t x67 = ffma2(pack_u2(sv[c][e + 6], sv[c][e + 7]), sl2_2, negm2);
-              float a0, a1, a2, a3, a4, a5, a6, a7;
-              unpack_f2(x01, a0, a1);
-              unpack_f2(x23, a2, a3);
-              unpack_f2(x45, a4, a5);
-              unpack_f2(x67, a6, a7);
-              const float p0 = exp2f(a0), p1 = exp2f(a1), p2 = exp2f(a2), p3 = exp2f(a3), p4 = exp2f(a4), p5 = exp2f(a5);
-              float p6, p7;
-              if (masked) {  // the polynomial gives 2^-126 where a masked score must give 0
-                p6 = exp2f(a6);
-                p7 = exp2f(a7);
-              } else {
-                unpack_f2(exp2_poly2(x67), p6, p7);
+              for (int u = 0; u < 4; ++u) x[u] = ffma2(pack_u2(s8[2 * u], s8[2 * u + 1]), sl2_2, negm2);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (decltype(poly)::value && u == 3) {
+                  p[u] = exp2_poly2(x[u]);
+                } else {
+                  float x0, x1;
+                  unpack_f2(x[u], x0, x1);
+                  p[u] = pack_f2(exp2f(x0), exp2f(x1));
+                }
               }
-              ls2 = fadd2(ls2, fadd2(fadd2(pack_f2(p0, p1), pack_f2(p2, p3)), fadd2(pack_f2(p4, p5), pack_f2(p6, p7))));
-              pk[cc * 16 + (e >> 1)] = pack_bf16(p0, p1);
-              pk[cc * 16 + (e >> 1) + 1] = pack_bf16(p2, p3);
-              pk[cc * 16 + (e >> 1) + 2] = pack_bf16(p4, p5);
-              pk[cc * 16 + (e >> 1) + 3] = pack_bf16(p6, p7);
+              ls2[g & 1] = fadd2(ls2[g & 1], fadd2(fadd2(p[0], p[1]), fadd2(p[2], p[3])));
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                float p0, p1;
+                unpack_f2(p[u], p0, p1);
+                pk[4 * g + u] = pack_bf16(p0, p1);
+              }
             }
+            tmem_st32(tSt + hf * 32, pk);
           }
-          tmem_st32(tSt + hf * 32, pk);
-        }
+        };
+        // the polynomial gives 2^-126 where a masked score must give 0
+        if (masked) exponentials(std::false_type{}); else exponentials(std::true_type{});
         {
           float s0, s1;
-          unpack_f2(ls2, s0, s1);
+          unpack_f2(fadd2(ls2[0], ls2[1]), s0, s1);
           l += s0 + s1;
         }
         // V rows that no row of the pair sees
@@ -575,7 +592,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         slot[256 * D + 256 + srow] = l;
       }
       tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_full, may overwrite it
-      if (!whole && i0 == 0 && threadIdx.x == 64) {
+      if (!whole && i0 == 0 && threadIdx.x == 128) {
         const long long end_unit = u1 - (i1 - i0) + t.nt - 1;  // last unit of this item
         long long i = (end_unit * n_blocks) / total;           // share it belongs to
         while (i + 1 < n_blocks && total * (i + 1) / n_blocks <= end_unit) ++i;
