@@ -18,7 +18,6 @@
 //  * Keys past the end of a sequence and behind the window lie in the same pages as visible ones. Their scores are
 //    replaced by -inf, and their V rows are zeroed in shared memory by the softmax threads before P is handed over (0 x NaN
 //    would reach every row). Pages that are missing are requested outside the pool, which TMA fills with zeros.
-#include <type_traits>
 #include "common.cuh"
 #include "lingua_b200.h"
 
@@ -113,7 +112,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   __shared__ uint32_t tmem_slot;
   __shared__ long long warp_sum[CK_THREADS / 32];
   __shared__ CkWalk start;
-  __shared__ __align__(8) uint64_t bar_mem[2 + 4 * NST + 6];
+  __shared__ __align__(8) uint64_t bar_mem[2 + 4 * NST + 8];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   auto sQ = [&](int t) { return sbase + t * Cfg::TILE; };
   auto sK = [&](int s) { return sbase + (2 + 2 * s) * Cfg::TILE; };
@@ -124,9 +123,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   auto v_full = [&](int s) { return bars + 24 + 32 * s; };
   auto k_empty = [&](int s) { return bars + 32 + 32 * s; };
   auto v_empty = [&](int s) { return bars + 40 + 32 * s; };
-  auto s_full = [&](int t) { return bars + 16 + 32 * NST + 24 * t; };
-  auto p_full = [&](int t) { return bars + 24 + 32 * NST + 24 * t; };
-  auto o_done = [&](int t) { return bars + 32 + 32 * NST + 24 * t; };
+  auto s_full = [&](int t) { return bars + 16 + 32 * NST + 32 * t; };
+  auto p_half = [&](int t) { return bars + 24 + 32 * NST + 32 * t; };
+  auto p_full = [&](int t) { return bars + 32 + 32 * NST + 32 * t; };
+  auto o_done = [&](int t) { return bars + 40 + 32 * NST + 32 * t; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hkv, tpt = 128 / G;
@@ -143,6 +143,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
+      mbar_init(p_half(t), 4);
       mbar_init(p_full(t), 4);
       mbar_init(o_done(t), 1);
     }
@@ -357,12 +358,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             umma_commit(s_full(s));
           };
           auto issue_pv = [&](int s, int st, int i) -> bool {
-            if (!mbar_wait(p_full(s), n_p[s] & 1, &abort_flag, a.status, 0x64)) return false;
-            tc_fence_after();
+              // the first 64 keys' P is multiplied while the softmax warps are still at the other 64
             const uint64_t dv = make_smem_desc(sV(st), CK_HALF, 1024);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ts(tO(s), tS(s) + k * 8, ck_slice_mn(dv, k), IDESC_O, (begun[s] || k != 0) ? 1u : 0u);
+            for (int hf = 0; hf < 2; ++hf) {
+              if (!mbar_wait(hf ? p_full(s) : p_half(s), n_p[s] & 1, &abort_flag, a.status, 0x64)) return false;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 4 * hf; k < 4 * hf + 4; ++k)
+                umma_f16_ts(tO(s), tS(s) + k * 8, ck_slice_mn(dv, k), IDESC_O, (begun[s] || k != 0) ? 1u : 0u);
+            }
             begun[s] = true;
             ++n_p[s];
             if (i == last[s]) umma_commit(o_done(s));
@@ -437,22 +442,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         tmem_wait_ld();
         const bool masked = k0 + 128 > min(p_first + 1, q.end) || (a.window > 0 && k0 < lo_last && k0 + 128 > a.sinks);
         if (masked) {
-          // key k0 + x is visible for x < up, and x >= down or x < top; every other score becomes -inf
-          const int up = hi - k0;
-          if (a.window > 0) {
-            const int down = lo - k0, top = a.sinks - k0;
+          // key k0 + x is visible for x < up, and x >= down or x < top; every other score becomes -inf. One bit mask per
+          // 32 keys: this path runs rarely, so its length (cold instruction cache) counts for more than its arithmetic.
+          const int up = hi - k0, down = a.window > 0 ? lo - k0 : 0, top = a.sinks - k0;
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t vis = below(up - 32 * c) & (~below(down - 32 * c) | below(top - 32 * c));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int x = c * 32 + e;
-                sv[c][e] = ((x < up) & ((x >= down) | (x < top))) ? sv[c][e] : 0xFF800000u;
-              }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sv[c][e] = c * 32 + e < up ? sv[c][e] : 0xFF800000u;
+            for (int e = 0; e < 32; ++e) sv[c][e] = (vis >> e) & 1 ? sv[c][e] : 0xFF800000u;
           }
         }
         float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -484,49 +482,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             if (need) m_used = m_new;
           }
         }
-        const float m_eff = m_used == -INFINITY ? 0.f : m_used;
-        // P = exp2(S scale - m) in bf16 (half a step, 2^-8 of each); the row sum is taken before that rounding. Two of
-        // eight exponentials run on the FMA pipe, so that the MUFU is not the limit.
-        const uint64_t sl2_2 = pack_f2(sl2, sl2), negm2 = pack_f2(-m_eff, -m_eff);
-        uint64_t ls2[2] = {0ull, 0ull};
-        auto exponentials = [&](auto poly) {  // one straight run of code per kind of tile: a branch in it would serialise it
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              const uint32_t* s8 = &sv[2 * hf + (g >> 2)][8 * (g & 3)];
-              uint64_t x[4], p[4];
-#pragma unroll
-              for (int u = 0; u < 4; ++u) x[u] = ffma2(pack_u2(s8[2 * u], s8[2 * u + 1]), sl2_2, negm2);
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                if (decltype(poly)::value && u == 3) {
-                  p[u] = exp2_poly2(x[u]);
-                } else {
-                  float x0, x1;
-                  unpack_f2(x[u], x0, x1);
-                  p[u] = pack_f2(exp2f(x0), exp2f(x1));
-                }
-              }
-              ls2[g & 1] = fadd2(ls2[g & 1], fadd2(fadd2(p[0], p[1]), fadd2(p[2], p[3])));
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                float p0, p1;
-                unpack_f2(p[u], p0, p1);
-                pk[4 * g + u] = pack_bf16(p0, p1);
-              }
-            }
-            tmem_st32(tSt + hf * 32, pk);
-          }
-        };
-        // the polynomial gives 2^-126 where a masked score must give 0
-        if (masked) exponentials(std::false_type{}); else exponentials(std::true_type{});
-        {
-          float s0, s1;
-          unpack_f2(fadd2(ls2[0], ls2[1]), s0, s1);
-          l += s0 + s1;
-        }
         // V rows that no row of the pair sees
         const int row_key = k0 + r;
         const bool edge = k0 + 128 > t.hi || (a.window > 0 && k0 < t.lo && k0 + 128 > a.sinks);
@@ -543,10 +498,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           }
           fence_proxy_async_smem();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(wt));
+        const float m_eff = m_used == -INFINITY ? 0.f : m_used;
+        // P = exp2(S scale - m) in bf16 (half a step, 2^-8 of each); the row sum is taken before that rounding. Two of
+        // eight exponentials run on the FMA pipe, so that the MUFU is not the limit; the polynomial gives 2^-126 for a
+        // masked score, which is nothing beside the row's largest (a row without any is caught at the end).
+        const uint64_t sl2_2 = pack_f2(sl2, sl2), negm2 = pack_f2(-m_eff, -m_eff);
+        uint64_t ls2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const uint32_t* s8 = &sv[2 * hf + (g >> 2)][8 * (g & 3)];
+            uint64_t x[4], p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = ffma2(pack_u2(s8[2 * u], s8[2 * u + 1]), sl2_2, negm2);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (u == 3) {
+                p[u] = exp2_poly2(x[u]);
+              } else {
+                float x0, x1;
+                unpack_f2(x[u], x0, x1);
+                p[u] = pack_f2(exp2f(x0), exp2f(x1));
+              }
+            }
+            ls2[g & 1] = fadd2(ls2[g & 1], fadd2(fadd2(p[0], p[1]), fadd2(p[2], p[3])));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              float p0, p1;
+              unpack_f2(p[u], p0, p1);
+              pk[4 * g + u] = pack_bf16(p0, p1);
+            }
+          }
+          tmem_st32(tSt + hf * 32, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(hf ? p_full(wt) : p_half(wt));
+        }
+        {
+          float s0, s1;
+          unpack_f2(fadd2(ls2[0], ls2[1]), s0, s1);
+          l += s0 + s1;
+        }
       }
       // ---- epilogue of the piece
       if (any) {
@@ -555,6 +550,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         tc_fence_after();
       }
       const bool whole = i0 == 0 && i1 == t.nt;
+      if (m_used == -INFINITY) l = 0.f;  // saw no key
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* orow = (__nv_bfloat16*)a.o + ((long long)(q.q0 + t.tok0 + wt * tpt + rt) * a.H + w.hk * G + rg) * D;
       float* slot = ws + (long long)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * Cfg::SLOT;
@@ -591,7 +587,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         slot[256 * D + srow] = m_used;
         slot[256 * D + 256 + srow] = l;
       }
-      tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_full, may overwrite it
+      tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_half, may overwrite it
       if (!whole && i0 == 0 && threadIdx.x == 128) {
         const long long end_unit = u1 - (i1 - i0) + t.nt - 1;  // last unit of this item
         long long i = (end_unit * n_blocks) / total;           // share it belongs to
