@@ -341,7 +341,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       });
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA
-      if (lane == 0) {
+      if (elect_one()) {
         uint32_t kv = 0, piece = 0, n_p[2] = {0, 0};
         walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
           int last[2] = {-1, -1};  // last active key tile of each query tile
