@@ -427,12 +427,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       const int pos = p_first + rt;
       const int hi = live ? max(0, min(pos + 1, q.end)) : 0;  // this row sees keys below hi ...
       const int lo = a.window > 0 ? pos - a.window + 1 : 0;   // ... from lo on, and the first `sinks`
-      const int lo_last = a.window > 0 ? p_first + n_tok - a.window : 0;
+      // key tiles inside [full_lo, full_hi) (or the first tokens) are seen by every row
+      const int full_hi = min(p_first + 1, q.end), full_lo = a.window > 0 ? p_first + n_tok - a.window : 0;
       float m_used = -INFINITY, l = 0.f;
       bool any = false;
       for (int i = i0; i < i1; ++i, ++kv) {
         const int kt = ck_tile(t, i), k0 = kt * 128;
         if (!ck_active(a, t, wt, kt)) continue;
+        const bool masked = k0 + 128 > full_hi || (k0 < full_lo && k0 + 128 > a.sinks);
         if (!wait_all(s_full(wt), n_s & 1, 0x68)) return false;
         ++n_s;
         tc_fence_after();
@@ -440,7 +442,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tSt + c * 32, sv[c]);
         tmem_wait_ld();
-        const bool masked = k0 + 128 > min(p_first + 1, q.end) || (a.window > 0 && k0 < lo_last && k0 + 128 > a.sinks);
         if (masked) {
           // key k0 + x is visible for x < up, and x >= down or x < top; every other score becomes -inf. One bit mask per
           // 32 keys: this path runs rarely, so its length (cold instruction cache) counts for more than its arithmetic.
@@ -452,14 +453,31 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 #pragma unroll
             for (int e = 0; e < 32; ++e) sv[c][e] = (vis >> e) & 1 ? sv[c][e] : 0xFF800000u;
           }
+          // V rows that no row of the pair sees (such tiles are masked ones)
+          if (k0 + 128 > t.hi || (k0 < t.lo && k0 + 128 > a.sinks)) {
+            const int key = k0 + r;
+            const uint32_t st = kv % NST;
+            if (!wait_all(v_full(st), (kv / NST) & 1, 0x69)) return false;
+            if (key >= t.hi || (key < t.lo && key >= a.sinks)) {
+#pragma unroll
+              for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sV(st) + h * CK_HALF + r * 128 + u * 16), "r"(0)
+                               : "memory");
+            }
+            fence_proxy_async_smem();
+          }
         }
-        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mxa[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int u = 0; u < 8; ++u) mxa[u] = fmaxf(__uint_as_float(sv[0][u]), __uint_as_float(sv[0][u + 8]));
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            mxa[(e >> 1) & 3] = fmax3(mxa[(e >> 1) & 3], __uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1]));
-        const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * sl2;
+        for (int x = 16; x < 128; x += 16)
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            mxa[u] = fmax3(mxa[u], __uint_as_float(sv[x >> 5][(x & 31) + u]), __uint_as_float(sv[x >> 5][(x & 31) + 8 + u]));
+        const float mx = fmaxf(fmax3(mxa[0], mxa[1], mxa[2]), fmax3(fmax3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7])) * sl2;
         const float m_new = fmaxf(m_used, mx);
         if (!any) {
           m_used = m_new;
@@ -482,26 +500,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             if (need) m_used = m_new;
           }
         }
-        // V rows that no row of the pair sees
-        const int row_key = k0 + r;
-        const bool edge = k0 + 128 > t.hi || (a.window > 0 && k0 < t.lo && k0 + 128 > a.sinks);
-        if (edge) {
-          const uint32_t st = kv % NST;
-          if (!wait_all(v_full(st), (kv / NST) & 1, 0x69)) return false;
-          if (row_key >= t.hi || (row_key < t.lo && row_key >= a.sinks)) {
-#pragma unroll
-            for (int h = 0; h < NH; ++h)
-#pragma unroll
-              for (int u = 0; u < 8; ++u)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sV(st) + h * CK_HALF + r * 128 + u * 16), "r"(0)
-                             : "memory");
-          }
-          fence_proxy_async_smem();
-        }
         const float m_eff = m_used == -INFINITY ? 0.f : m_used;
-        // P = exp2(S scale - m) in bf16 (half a step, 2^-8 of each); the row sum is taken before that rounding. Two of
-        // eight exponentials run on the FMA pipe, so that the MUFU is not the limit; the polynomial gives 2^-126 for a
-        // masked score, which is nothing beside the row's largest (a row without any is caught at the end).
+        // P = exp2(S scale - m) in bf16 (half a step, 2^-8 of each); the row sum is taken before that rounding. All on the
+        // MUFU: a polynomial for a part of them on the FMA pipe lengthened the one thread's run that the other tile's
+        // products have to cover (0 / 1 / 2 / 3 / 4 of 8 by polynomial: 878 / 898 / 894 / 909 / 933 us for 2048 tokens
+        // over 32768 keys).
         const uint64_t sl2_2 = pack_f2(sl2, sl2), negm2 = pack_f2(-m_eff, -m_eff);
         uint64_t ls2[2] = {0ull, 0ull};
 #pragma unroll
@@ -515,13 +518,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             for (int u = 0; u < 4; ++u) x[u] = ffma2(pack_u2(s8[2 * u], s8[2 * u + 1]), sl2_2, negm2);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-              if (u == 3) {
-                p[u] = exp2_poly2(x[u]);
-              } else {
-                float x0, x1;
-                unpack_f2(x[u], x0, x1);
-                p[u] = pack_f2(exp2f(x0), exp2f(x1));
-              }
+              float x0, x1;
+              unpack_f2(x[u], x0, x1);
+              p[u] = pack_f2(exp2f(x0), exp2f(x1));
             }
             ls2[g & 1] = fadd2(ls2[g & 1], fadd2(fadd2(p[0], p[1]), fadd2(p[2], p[3])));
 #pragma unroll
@@ -550,7 +549,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         tc_fence_after();
       }
       const bool whole = i0 == 0 && i1 == t.nt;
-      if (m_used == -INFINITY) l = 0.f;  // saw no key
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* orow = (__nv_bfloat16*)a.o + ((long long)(q.q0 + t.tok0 + wt * tpt + rt) * a.H + w.hk * G + rg) * D;
       float* slot = ws + (long long)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * Cfg::SLOT;
