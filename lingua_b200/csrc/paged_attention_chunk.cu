@@ -36,7 +36,7 @@ struct CkCfg {
   static constexpr int NH = D / 64;           // 64-channel halves of a row
   static constexpr int TILE = NH * CK_HALF;   // 128 rows x D
   static constexpr int NST = D == 128 ? 2 : 4;
-  static constexpr int SMEM = 2 * TILE + 2 * NST * TILE + 1024;
+  static constexpr int SMEM = 2 * TILE + 2 * NST * TILE + 8 * 2048 /* output staging of a softmax warp */ + 1024;
   static constexpr int SLOT = 256 * D + 512;  // floats of a partial result: O, row maxima, row sums
 };
 
@@ -417,6 +417,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tSt = tS(wt) + lane_off, tOt = tO(wt) + lane_off;
+    const uint32_t stage = sbase + (2 + 2 * NST) * Cfg::TILE + (warp - 4) * 2048;
     const float sl2 = fmaxf(a.scale * CK_LOG2E, 1e-30f);  // a scale of 0 must not turn -inf into NaN
     const int rt = r / G, rg = r % G;  // token and head of this row
     uint32_t kv = 0, n_s = 0, n_o = 0;
@@ -549,41 +550,74 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         tc_fence_after();
       }
       const bool whole = i0 == 0 && i1 == t.nt;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* orow = (__nv_bfloat16*)a.o + ((long long)(q.q0 + t.tok0 + wt * tpt + rt) * a.H + w.hk * G + rg) * D;
-      float* slot = ws + (long long)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * Cfg::SLOT;
-      const int srow = wt * 128 + r;
+      if (whole) {
+        // 32 columns at a time through shared memory, so that a store instruction writes 8 rows of 64 bytes instead of
+        // 32 rows of 16 (rows of o lie H x D elements apart for every token)
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        unsigned long long out = 0;  // address of this row of o, 0: no such row
+        if (live) out = (unsigned long long)((__nv_bfloat16*)a.o +
+                                             ((long long)(q.q0 + t.tok0 + wt * tpt + rt) * a.H + w.hk * G + rg) * D);
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t rr[32];
-        if (any) {
-          tmem_ld32(tOt + c * 32, rr);
-          tmem_wait_ld();
-        } else {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t rr[32];
+          if (any) {
+            tmem_ld32(tOt + c * 32, rr);
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) rr[e] = 0u;
-        }
-        if (whole && live) {
+            for (int e = 0; e < 32; ++e) rr[e] = 0u;
+          }
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            uint4 v;
-            v.x = pack_bf16(__uint_as_float(rr[g * 8 + 0]) * inv, __uint_as_float(rr[g * 8 + 1]) * inv);
-            v.y = pack_bf16(__uint_as_float(rr[g * 8 + 2]) * inv, __uint_as_float(rr[g * 8 + 3]) * inv);
-            v.z = pack_bf16(__uint_as_float(rr[g * 8 + 4]) * inv, __uint_as_float(rr[g * 8 + 5]) * inv);
-            v.w = pack_bf16(__uint_as_float(rr[g * 8 + 6]) * inv, __uint_as_float(rr[g * 8 + 7]) * inv);
-            *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) = v;
+            const uint32_t x0 = pack_bf16(__uint_as_float(rr[g * 8 + 0]) * inv, __uint_as_float(rr[g * 8 + 1]) * inv);
+            const uint32_t x1 = pack_bf16(__uint_as_float(rr[g * 8 + 2]) * inv, __uint_as_float(rr[g * 8 + 3]) * inv);
+            const uint32_t x2 = pack_bf16(__uint_as_float(rr[g * 8 + 4]) * inv, __uint_as_float(rr[g * 8 + 5]) * inv);
+            const uint32_t x3 = pack_bf16(__uint_as_float(rr[g * 8 + 6]) * inv, __uint_as_float(rr[g * 8 + 7]) * inv);
+            // piece g of row `lane`; the exclusive or spreads the rows of a quarter warp over the banks
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)),
+                         "r"(x0), "r"(x1), "r"(x2), "r"(x3)
+                         : "memory");
           }
-        } else if (live) {
+          __syncwarp();
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            *reinterpret_cast<uint4*>(slot + srow * D + c * 32 + g * 4) =
-                make_uint4(rr[4 * g], rr[4 * g + 1], rr[4 * g + 2], rr[4 * g + 3]);
+          for (int g = 0; g < 4; ++g) {
+            const int row = g * 8 + (lane >> 2), piece = lane & 3;
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                         : "memory");
+            const unsigned long long to = __shfl_sync(0xFFFFFFFFu, out, row);
+            if (to) *reinterpret_cast<uint4*>(to + c * 64 + piece * 16) = v;
+          }
+          __syncwarp();
         }
-        __syncwarp();
-      }
-      if (!whole && live) {
-        slot[256 * D + srow] = m_used;
-        slot[256 * D + 256 + srow] = l;
+      } else {
+        // partial result: vectors of four columns, each for all 256 rows of the pair side by side
+        float* slot = ws + (long long)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * Cfg::SLOT;
+        const int srow = wt * 128 + r;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t rr[32];
+          if (any) {
+            tmem_ld32(tOt + c * 32, rr);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) rr[e] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              *reinterpret_cast<uint4*>(slot + ((c * 8 + g) * 256 + srow) * 4) =
+                  make_uint4(rr[4 * g], rr[4 * g + 1], rr[4 * g + 2], rr[4 * g + 3]);
+          }
+          __syncwarp();
+        }
+        if (live) {
+          slot[256 * D + srow] = m_used;
+          slot[256 * D + 256 + srow] = l;
+        }
       }
       tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_half, may overwrite it
       if (!whole && i0 == 0 && threadIdx.x == 128) {
@@ -610,39 +644,53 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   }
 }
 
-// Joins the parts of the item that block blockIdx.x began and later blocks went on with; a warp per row.
+// Joins the parts of the item that block blockIdx.x began and later blocks went on with: a thread per row of the pair,
+// blockIdx.y takes 8 columns.
 template <int D>
 __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const LbPagedAttnArgs a, const float* ws, const int4* hdr) {
   using Cfg = CkCfg<D>;
-  constexpr int E = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 h = hdr[blockIdx.x];
   if (h.w == 0) return;
   const int G = a.H / a.Hkv, tpt = 128 / G;
   const CkSeq q = ck_seq(a, h.x, false);
-  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int r = row & 127, tok = h.z * 2 * tpt + (row >> 7) * tpt + r / G;
+  const int row = threadIdx.x, r = row & 127, tok = h.z * 2 * tpt + (row >> 7) * tpt + r / G;
   if (r >= tpt * G || tok >= q.nq) return;
-  float m = -INFINITY, l = 0.f, o[E];
+  auto slot = [&](int part) { return ws + (long long)(part == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + part)) * Cfg::SLOT; };
+  float m = -INFINITY, l = 0.f;
+  float4 o[2];
+  o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int part = 0; part < h.w; part += 4) {  // four parts' loads in flight
+    float pm[4], pl[4];
+    float4 x[4][2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int part = 0; part < h.w; ++part) {
-    const float* p = ws + (long long)(part == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + part)) * Cfg::SLOT;
-    const float pm = p[256 * D + row], pl = p[256 * D + 256 + row];
-    float x[E];
+    for (int u = 0; u < 4; ++u) {
+      const float* p = slot(min(part + u, h.w - 1));
+      pm[u] = part + u < h.w ? p[256 * D + row] : -INFINITY;
+      pl[u] = p[256 * D + 256 + row];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = p[row * D + lane * E + e];
-    const float mn = fmaxf(m, pm);
-    const float fa = m == -INFINITY ? 0.f : exp2f(m - mn), fb = pm == -INFINITY ? 0.f : exp2f(pm - mn);
+      for (int g = 0; g < 2; ++g) x[u][g] = *reinterpret_cast<const float4*>(p + ((blockIdx.y * 2 + g) * 256 + row) * 4);
+    }
+    const float mn = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
+    const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn);
     m = mn;
-    l = l * fa + pl * fb;
+    l *= f0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * fa + x[e] * fb;
+    for (int g = 0; g < 2; ++g) { o[g].x *= f0; o[g].y *= f0; o[g].z *= f0; o[g].w *= f0; }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = pm[u] == -INFINITY ? 0.f : exp2f(pm[u] - mn);
+      l += f * pl[u];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        o[g].x += f * x[u][g].x; o[g].y += f * x[u][g].y; o[g].z += f * x[u][g].z; o[g].w += f * x[u][g].w;
+      }
+    }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  __nv_bfloat16* dst = (__nv_bfloat16*)a.o + ((long long)(q.q0 + tok) * a.H + h.y * G + r % G) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(o[e] * inv, o[e + 1] * inv);
+  *reinterpret_cast<uint4*>((__nv_bfloat16*)a.o + ((long long)(q.q0 + tok) * a.H + h.y * G + r % G) * D + blockIdx.y * 8) =
+      make_uint4(pack_bf16(o[0].x * inv, o[0].y * inv), pack_bf16(o[0].z * inv, o[0].w * inv),
+                 pack_bf16(o[1].x * inv, o[1].y * inv), pack_bf16(o[1].z * inv, o[1].w * inv));
 }
 
 template <int D>
@@ -662,7 +710,7 @@ static int launch_chunk(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
   paged_chunk_kernel<D><<<grid, CK_THREADS, Cfg::SMEM, st>>>(tq, tk, tv, a, (float*)ws, hdr);
   g_launches.fetch_add(1, std::memory_order_relaxed);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 32);
+  cfg.gridDim = dim3(grid, D / 8);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
