@@ -4,8 +4,8 @@
 // 2 x 128 x D x 2 bytes of keys and values that 256 rows share. What the design follows from:
 //  * The rows of a query tile are (token, query head of one kv head) pairs: 128 / G tokens x G heads, loaded by one TMA box.
 //    A key tile is thus fetched once for all heads of the group, and short chunks of grouped heads still fill tiles.
-//  * An item is (sequence, kv head, pair of query tiles). Its key tiles of 128 (the visible ones only) are dealt out, all
-//    items in order, in equal contiguous shares to one block per SM. A share that begins or ends inside an item leaves a
+//  * An item is (sequence, kv head, pair of query tiles). Its units, CK_ITEM_COST for the item itself and one for each visible
+//    key tile of 128, are dealt out, all items in order, in equal contiguous shares to one block per SM. A share that begins or ends inside an item leaves a
 //    partial result (row maximum, row sum, unnormalised output in fp32) for the join kernel at the end. So one long chunk
 //    of few heads, a batch of odd chunks and a whole prompt all keep 148 SMs equally busy.
 //  * Each query tile of the pair has its own softmax warpgroup (a thread owns a whole row of 128 scores, no exchange between
@@ -28,6 +28,7 @@ namespace lb {
 // 128 x 88 + 256 x 208).
 constexpr int CK_THREADS = 384;
 constexpr int CK_REGS_CONTROL = 88, CK_REGS_SOFTMAX = 208;
+constexpr int CK_ITEM_COST = 3;     // what beginning and ending an item costs, in key tiles (about 5 us against 1.9 us)
 constexpr int CK_HALF = 128 * 128;  // 128 rows x 64 channels: one swizzled box of a tile
 constexpr float CK_LOG2E = 1.4426950408889634f;
 
@@ -36,9 +37,14 @@ struct CkCfg {
   static constexpr int NH = D / 64;           // 64-channel halves of a row
   static constexpr int TILE = NH * CK_HALF;   // 128 rows x D
   static constexpr int NST = D == 128 ? 2 : 4;
-  static constexpr int SMEM = 2 * TILE + 2 * NST * TILE + 8 * 2048 /* output staging of a softmax warp */ + 1024;
+  static constexpr int SMEM = 2 * TILE + 2 * NST * TILE + 8 * 4096 /* output staging of a softmax warp */ + 1024;
   static constexpr int SLOT = 256 * D + 512;  // floats of a partial result: O, row maxima, row sums
 };
+
+// a / b of non-negative numbers; 64-bit division is a long subroutine
+__device__ __forceinline__ long long ck_div(long long a, long long b) {
+  return (unsigned long long)a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 
 struct CkSeq {
   int q0, nq, pos0, end;  // first row of q, new tokens, position of the first one, end of the readable keys
@@ -91,8 +97,8 @@ __device__ __forceinline__ bool ck_active(const LbPagedAttnArgs& a, const CkItem
 
 // A block's place in the list of items; every role of the block walks it the same way.
 struct CkWalk {
-  int seq, hk, pair, first;  // item and the first of its key tiles that is this block's
-  long long left;            // key tiles still to do
+  int seq, hk, pair, first;  // item and the first of its units that is this block's
+  long long left;            // units still to do
 };
 
 // Descriptors of the k-th 16-deep slice of a tile: the start address (in units of 16 bytes, the low field) moves by
@@ -169,7 +175,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   auto seq_tiles = [&](const CkSeq& q) {  // of one kv head; the same in all lanes
     const int n_pairs = (q.nq + 2 * tpt - 1) / (2 * tpt);
     long long n = 0;
-    for (int p = lane; p < n_pairs; p += 32) n += ck_item(a, q, p, tpt).nt;
+    for (int p = lane; p < n_pairs; p += 32) n += ck_item(a, q, p, tpt).nt + CK_ITEM_COST;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
     return n;
@@ -202,7 +208,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   }
   const long long n_blocks = max(1ll, min((long long)gridDim.x, total));  // no share is empty
   const bool busy = blockIdx.x < n_blocks;
-  const long long u0 = busy ? total * blockIdx.x / n_blocks : 0, u1 = busy ? total * (blockIdx.x + 1) / n_blocks : 0;
+  auto share = [&](long long i) { return ck_div(total * i, n_blocks); };  // first unit of share i
+  const long long u0 = busy ? share(blockIdx.x) : 0, u1 = busy ? share(blockIdx.x + 1) : 0;
   if (u0 < u1 && u0 >= before && u0 < before + mine) {
     long long at = before;
     bool found = false;
@@ -215,11 +222,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         const long long one = seq_tiles(q);
         if (u0 < at + a.Hkv * one) {
           found = true;
-          const int hk = (int)((u0 - at) / one);
-          long long rest = (u0 - at) % one;  // key tiles of this head before u0
+          const int hk = (int)ck_div(u0 - at, one);
+          long long rest = u0 - at - hk * one;  // units of this head before u0
           const int n_pairs = (q.nq + 2 * tpt - 1) / (2 * tpt);
           for (int p0 = 0; p0 < n_pairs; p0 += 32) {
-            const int nt = p0 + lane < n_pairs ? ck_item(a, q, p0 + lane, tpt).nt : 0;
+            const int nt = p0 + lane < n_pairs ? ck_item(a, q, p0 + lane, tpt).nt + CK_ITEM_COST : 0;
             long long incl = nt;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -273,9 +280,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         continue;
       }
       const CkItem t = ck_item(a, q, w.pair, tpt);
-      const int i1 = (int)min((long long)t.nt, w.first + w.left);
-      if (!body(q, t, w, w.first, i1)) return;
-      w.left -= i1 - w.first;
+      const int f1 = (int)min((long long)(t.nt + CK_ITEM_COST), w.first + w.left);
+      const int i0 = max(0, w.first - CK_ITEM_COST), i1 = max(0, f1 - CK_ITEM_COST);
+      if (i1 > i0 && !body(q, t, w, i0, i1)) return;
+      w.left -= f1 - w.first;
       w.first = 0;
       ++w.pair;
     }
@@ -310,14 +318,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           return pg;
         };
         int pg = page_of(i0);
-        if (!wait_all(q_empty, (piece & 1) ^ 1, 0x61)) return false;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, (t.n_tok1 > 0 ? 2 : 1) * q_bytes);
-          for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
-            for (int h = 0; h < NH; ++h)
-              tma_load_4d(sQ(s) + h * CK_HALF, &tq, q_full, 64 * h, w.hk * G, q.q0 + t.tok0 + s * tpt, 0);
-        }
-        ++piece;
         for (int i = i0; i < i1; ++i, ++kv) {
           const int s = kv % NST;
           const uint32_t ph = ((kv / NST) & 1) ^ 1;
@@ -336,6 +336,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             for (int h = 0; h < NH; ++h)
               tma_load_4d(sV(s) + h * CK_HALF + lane * rows * 128, &tv, v_full(s), 64 * h, off, w.hk, pg);
           pg = next;
+          if (i == i0) {  // after the first keys, whose stages come free earlier than the Q tiles
+            if (!wait_all(q_empty, (piece & 1) ^ 1, 0x61)) return false;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(q_full, (t.n_tok1 > 0 ? 2 : 1) * q_bytes);
+              for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
+                for (int h = 0; h < NH; ++h)
+                  tma_load_4d(sQ(s) + h * CK_HALF, &tq, q_full, 64 * h, w.hk * G, q.q0 + t.tok0 + s * tpt, 0);
+            }
+            ++piece;
+          }
         }
         return true;
       });
@@ -345,7 +355,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         uint32_t kv = 0, piece = 0, n_p[2] = {0, 0};
         walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
           int last[2] = {-1, -1};  // last active key tile of each query tile
-          for (int s = 0; s < 2; ++s)
+          for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
             for (int i = i1 - 1; i >= i0 && last[s] < 0; --i)
               if (ck_active(a, t, s, ck_tile(t, i))) last[s] = i;
           bool begun[2] = {false, false};
@@ -417,7 +427,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tSt = tS(wt) + lane_off, tOt = tO(wt) + lane_off;
-    const uint32_t stage = sbase + (2 + 2 * NST) * Cfg::TILE + (warp - 4) * 2048;
+    const uint32_t stage = sbase + (2 + 2 * NST) * Cfg::TILE + (warp - 4) * 4096;
     const float sl2 = fmaxf(a.scale * CK_LOG2E, 1e-30f);  // a scale of 0 must not turn -inf into NaN
     const int rt = r / G, rg = r % G;  // token and head of this row
     uint32_t kv = 0, n_s = 0, n_o = 0;
@@ -551,44 +561,45 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       }
       const bool whole = i0 == 0 && i1 == t.nt;
       if (whole) {
-        // 32 columns at a time through shared memory, so that a store instruction writes 8 rows of 64 bytes instead of
+        // 64 columns at a time through shared memory, so that a store instruction writes 4 rows of 128 bytes instead of
         // 32 rows of 16 (rows of o lie H x D elements apart for every token)
         const float inv = l > 0.f ? 1.f / l : 0.f;
         unsigned long long out = 0;  // address of this row of o, 0: no such row
         if (live) out = (unsigned long long)((__nv_bfloat16*)a.o +
                                              ((long long)(q.q0 + t.tok0 + wt * tpt + rt) * a.H + w.hk * G + rg) * D);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t rr[32];
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t rr[2][32];
           if (any) {
-            tmem_ld32(tOt + c * 32, rr);
+            tmem_ld32(tOt + c * 64, rr[0]);
+            tmem_ld32(tOt + c * 64 + 32, rr[1]);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) rr[e] = 0u;
+            for (int e = 0; e < 64; ++e) rr[e >> 5][e & 31] = 0u;
           }
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const uint32_t x0 = pack_bf16(__uint_as_float(rr[g * 8 + 0]) * inv, __uint_as_float(rr[g * 8 + 1]) * inv);
-            const uint32_t x1 = pack_bf16(__uint_as_float(rr[g * 8 + 2]) * inv, __uint_as_float(rr[g * 8 + 3]) * inv);
-            const uint32_t x2 = pack_bf16(__uint_as_float(rr[g * 8 + 4]) * inv, __uint_as_float(rr[g * 8 + 5]) * inv);
-            const uint32_t x3 = pack_bf16(__uint_as_float(rr[g * 8 + 6]) * inv, __uint_as_float(rr[g * 8 + 7]) * inv);
+          for (int g = 0; g < 8; ++g) {
+            const uint32_t* x = &rr[g >> 2][(g & 3) * 8];
+            uint32_t y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y[u] = pack_bf16(__uint_as_float(x[2 * u]) * inv, __uint_as_float(x[2 * u + 1]) * inv);
             // piece g of row `lane`; the exclusive or spreads the rows of a quarter warp over the banks
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)),
-                         "r"(x0), "r"(x1), "r"(x2), "r"(x3)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((g ^ (lane & 7)) << 4)),
+                         "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
                          : "memory");
           }
           __syncwarp();
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int row = g * 8 + (lane >> 2), piece = lane & 3;
+          for (int g = 0; g < 8; ++g) {
+            const int row = g * 4 + (lane >> 3), piece = lane & 7;
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                         : "r"(stage + row * 128 + ((piece ^ (row & 7)) << 4))
                          : "memory");
             const unsigned long long to = __shfl_sync(0xFFFFFFFFu, out, row);
-            if (to) *reinterpret_cast<uint4*>(to + c * 64 + piece * 16) = v;
+            if (to) *reinterpret_cast<uint4*>(to + c * 128 + piece * 16) = v;
           }
           __syncwarp();
         }
@@ -621,10 +632,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       }
       tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_half, may overwrite it
       if (!whole && i0 == 0 && threadIdx.x == 128) {
-        const long long end_unit = u1 - (i1 - i0) + t.nt - 1;  // last unit of this item
-        long long i = (end_unit * n_blocks) / total;           // share it belongs to
-        while (i + 1 < n_blocks && total * (i + 1) / n_blocks <= end_unit) ++i;
-        while (i > 0 && total * i / n_blocks > end_unit) --i;
+        const long long end_unit = u1 - w.left - w.first + t.nt + CK_ITEM_COST - 1;  // last unit of this item
+        long long i = ck_div(end_unit * n_blocks, total);           // share it belongs to
+        while (i + 1 < n_blocks && share(i + 1) <= end_unit) ++i;
+        while (i > 0 && share(i) > end_unit) --i;
         hdr[blockIdx.x] = make_int4(w.seq, w.hk, w.pair, (int)(i - blockIdx.x + 1));
       }
       return true;
