@@ -526,12 +526,20 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
 }  // namespace lb
 
 namespace lb {
-// Up to CHUNK_ROWS rows (new tokens x heads of a group) a sequence's keys pass through the few-token kernel once or twice;
-// beyond that the tcgen05 kernel, which needs one pass for 256 rows, is faster.
+// The few-token kernel passes over a sequence's keys once for every 16 rows (new tokens x heads of a group), the tcgen05
+// kernel once for 256. Measured (8 kv heads, bf16, 128 channels, us, few-token / tcgen05): 16 rows 45 / 51 (1 sequence of
+// 32768 keys), 369 / 383 (64 of 8192), 116 / 156 (256 of 500); 32 rows 72 / 51, 694 / 385, 186 / 160. With little work for
+// each block the few-token kernel's shorter start decides: 1 sequence of 2000 keys 18 / 27 at 32 rows, 23 / 27 at 64,
+// 27 / 27 at 128; 300 keys 14 / 18.
 constexpr int CHUNK_ROWS = 16;
+constexpr int FEW_BLOCKS = 8;  // 64-key blocks for a thread block of the few-token kernel
 static bool use_chunk(const LbPagedAttnArgs& a) {
   const int G = a.H / a.Hkv;
-  return a.cu_q && G <= 128 && (long long)a.max_q * G > CHUNK_ROWS;
+  const long long rows = (long long)a.max_q * G;
+  if (!a.cu_q || G > 128 || rows <= CHUNK_ROWS) return false;
+  const long long blocks = (long long)a.n_seqs * a.Hkv * ((rows + DEC_ROWS - 1) / DEC_ROWS) *
+                           (((long long)a.cols * a.page + DEC_BLOCK - 1) / DEC_BLOCK);
+  return blocks > 2ll * num_sms() * FEW_BLOCKS;
 }
 }  // namespace lb
 

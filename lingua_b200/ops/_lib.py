@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -70,29 +71,11 @@ class AttnArgs(C.Structure):
     ]
 
 
-class PagedAppendArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_pages", "v_pages", "table", "kv_len", "cu_q", "cs",
-                                          "status")]
-    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "cs_rows")]
-    _fields_ += [(n, C.c_longlong) for n in ("table_stride", "q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "kp_sp",
-                                             "kp_st", "kp_sh", "vp_sp", "vp_st", "vp_sh")]
-
-
-class PagedAttnArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k_pages", "v_pages", "o", "table", "kv_len", "cu_q", "status")]
-    _fields_ += [(n, C.c_int) for n in ("T", "n_seqs", "H", "Hkv", "D", "page", "n_pages", "cols", "window", "sinks",
-                                         "max_q")]
-    _fields_ += [("scale", C.c_float)]
-    _fields_ += [(n, C.c_longlong) for n in ("table_stride", "q_st", "q_sh", "kp_sp", "kp_st", "kp_sh", "vp_sp", "vp_st",
-                                             "vp_sh")]
-
-
-class PenalizeArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("logits", "out", "history", "history_len", "prompt_len", "repetition", "presence",
-                                          "frequency", "bias", "allowed")]
-    _fields_ += [(n, C.c_int) for n in ("N", "V", "L", "dtype")]
-    _fields_ += [(n, C.c_float) for n in ("repetition_s", "presence_s", "frequency_s")]
-    _fields_ += [(n, C.c_longlong) for n in ("ld_in", "ld_out", "history_stride", "bias_stride", "allowed_stride")]
+# Argument blocks of the paged-cache and logits entry points, packed as the C structs of the same names (csrc/lingua_b200.h):
+# a ctypes.Structure takes several microseconds to fill, which is as long as the smallest of these kernels runs.
+PAGED_APPEND_ARGS = struct.Struct("@11P9i13q")  # LbPagedAppendArgs
+PAGED_ATTN_ARGS = struct.Struct("@8P11if9q")  # LbPagedAttnArgs
+PENALIZE_ARGS = struct.Struct("@10P4i3f5q")  # LbPenalizeArgs
 
 
 def lib_path() -> Path:
@@ -163,10 +146,10 @@ def _declare(lib) -> None:
         "lb_scan_fwd": [vp, vp, ip, fp, vp, fp, fp, i, i, i, vp],
         "lb_scan_bwd": [vp, vp, vp, ip, fp, vp, vp, fp, i, i, i, vp],
         "lb_decode_attn": [vp, vp, vp, vp, vp, ip, ip, vp, i, i, i, i, ll, ll, f, vp],
-        "lb_paged_append": [C.POINTER(PagedAppendArgs), vp],
-        "lb_paged_attention": [C.POINTER(PagedAttnArgs), vp, vp],
+        "lb_paged_append": [vp, vp],
+        "lb_paged_attention": [vp, vp, vp],
         "lb_copy_pages": [vp, ll, ll, ll, i, i, ip, ip, i, vp, vp],
-        "lb_penalize_logits": [C.POINTER(PenalizeArgs), vp],
+        "lb_penalize_logits": [vp, vp],
         "lb_conv1d_update": [vp, ll, vp, vp, vp, ll, i, i, i, i, vp],
         "lb_conv_states": [vp, ll, llp, llp, vp, i, i, i, vp],
         "lb_ssm_state_update": [fp, vp, ll, fp, fp, vp, ll, vp, ll, fp, i, vp, i, i, i, i, i, vp],
@@ -175,7 +158,7 @@ def _declare(lib) -> None:
         "lb_rglru_gates_bwd": [vp, vp, vp, fp, vp, vp, vp, vp, vp, fp, ll, i, vp],
     }
     if hasattr(lib, "lb_paged_attention_workspace"):
-        lib.lb_paged_attention_workspace.argtypes = [C.POINTER(PagedAttnArgs)]
+        lib.lb_paged_attention_workspace.argtypes = [C.c_void_p]
         lib.lb_paged_attention_workspace.restype = C.c_longlong
     for name, args in sigs.items():
         if hasattr(lib, name):
@@ -185,7 +168,7 @@ def _declare(lib) -> None:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def status_word(device=None) -> torch.Tensor:

@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .paged import _launch, _refuse
+from .paged import _on, _refuse
 
 Knob = Optional[Union[float, torch.Tensor]]
 
@@ -91,17 +91,16 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
     for t in (logits, history, history_len, prompt_len, bias, allowed, out):
         _refuse(t is not None and t.shape[-1] > 1 and t.stride(-1) != 1, "rows must be contiguous")
     if out is None:
-        out = torch.empty(N, V, dtype=logits.dtype, device=dev)
+        out = torch.empty((N, V), dtype=logits.dtype, device=dev)
     if N == 0 or V == 0:
         return out
-    def p(t):
-        return None if t is None else t.data_ptr()
-
-    a = _lib.PenalizeArgs(
-        logits.data_ptr(), out.data_ptr(), history.data_ptr(), history_len.data_ptr(), p(prompt_len), p(rep_t), p(pres_t),
-        p(freq_t), p(bias), p(allowed), N, V, history.shape[1],
-        _lib.LB_BF16 if logits.dtype == torch.bfloat16 else _lib.LB_F32, rep, pres, freq,
+    args = _lib.PENALIZE_ARGS.pack(
+        logits.data_ptr(), out.data_ptr(), history.data_ptr(), history_len.data_ptr(),
+        *(0 if t is None else t.data_ptr() for t in (prompt_len, rep_t, pres_t, freq_t, bias, allowed)), N, V,
+        history.shape[1], _lib.LB_BF16 if logits.dtype == torch.bfloat16 else _lib.LB_F32, rep, pres, freq,
         logits.stride(0), out.stride(0), history.stride(0), 0 if bias is None or bias.dim() == 1 else bias.stride(0),
         0 if allowed is None else allowed.stride(0))
-    _launch(_lib.load().lb_penalize_logits, a, dev, "lb_penalize_logits")
+    with _on(logits.get_device()):
+        rc = _lib.load().lb_penalize_logits(args, _lib.stream_ptr())
+    _lib.check(rc, "lb_penalize_logits")
     return out

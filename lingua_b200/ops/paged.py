@@ -16,7 +16,6 @@ apps/main/generate.py:299-320.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from contextlib import nullcontext
 from typing import Optional
@@ -43,7 +42,35 @@ def _strided(t: torch.Tensor, name: str) -> None:
     _refuse(not ok, f"{name} needs contiguous channels, 16-byte aligned rows and positive strides, got {tuple(st)}")
 
 
+def _aligned(t: torch.Tensor) -> bool:
+    """What ``_strided`` asks for, without the explanation."""
+    if t.data_ptr() % 16 or t.stride(-1) != 1:
+        return False
+    if t.is_contiguous():
+        return t.shape[-1] % 8 == 0
+    return all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
 def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
+    """One pass over the conditions; ``_refuse_cache`` finds the words when one fails."""
+    dev, dt, i32 = q.get_device(), q.dtype, torch.int32
+    if (q.dim() == 3 and k_pages.dim() == 4 and block_table.dim() == 2 and dev >= 0 and dt is torch.bfloat16):
+        n_pages, P, Hkv, D = shape = k_pages.shape
+        n = block_table.shape[0]
+        if (shape == v_pages.shape and q.shape[2] == D and D in HEAD_DIMS and P in PAGE_SIZES and n_pages > 0 and Hkv > 0
+                and q.shape[1] > 0 and q.shape[1] % Hkv == 0 and k_pages.dtype is dt and v_pages.dtype is dt
+                and block_table.dtype is i32 and kv_len.dtype is i32 and kv_len.shape == (n,)
+                and k_pages.get_device() == dev and v_pages.get_device() == dev and block_table.get_device() == dev
+                and kv_len.get_device() == dev and kv_len.is_contiguous()
+                and (q.shape[0] == n if cu_q is None else cu_q.dtype is i32 and cu_q.shape == (n + 1,)
+                     and cu_q.get_device() == dev and cu_q.is_contiguous())
+                and (block_table.stride(1) == 1 or block_table.shape[1] <= 1) and _aligned(q) and _aligned(k_pages)
+                and _aligned(v_pages) and not (q.requires_grad and torch.is_grad_enabled())):
+            return
+    _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
+
+
+def _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
     _refuse(q.dim() != 3, "new tokens are packed rows [T, heads, D]")
     _refuse(k_pages.dim() != 4 or k_pages.shape != v_pages.shape, "k_pages and v_pages must both be [n_pages, page, Hkv, D]")
     H, D, Hkv = q.shape[1], q.shape[2], k_pages.shape[2]
@@ -71,29 +98,24 @@ def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
     _refuse(not kv_len.is_contiguous() or (cu_q is not None and not cu_q.is_contiguous())
             or (block_table.shape[1] > 1 and block_table.stride(1) != 1), "kv_len, cu_q and table rows must be contiguous")
     _strided(q, "q")
-    if not k_pages.is_contiguous() or k_pages.data_ptr() % 16:
-        _strided(k_pages, "k_pages")
-    if not v_pages.is_contiguous() or v_pages.data_ptr() % 16:
-        _strided(v_pages, "v_pages")
+    _strided(k_pages, "k_pages")
+    _strided(v_pages, "v_pages")
 
 
-def _on(device: torch.device):
+_HERE = nullcontext()
+
+
+def _on(index: int):
     """Work on the operands' device, on that device's current stream, whichever device is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def _launch(fn, args, device: torch.device, what: str) -> None:
-    with _on(device):
-        rc = fn(C.byref(args), _lib.stream_ptr())
-    _lib.check(rc, what)
-
-
-def _status(device: torch.device) -> int:
-    t = _lib._status.get(device.index)
+def _status(index: int) -> int:
+    t = _lib._status.get(index)
     if t is None:
         # made here it would live in the graph's private memory and die with the graph
         _refuse(torch.cuda.is_current_stream_capturing(), "call a paged-cache operator once before capturing it into a graph")
-        t = _lib.status_word(device)
+        t = _lib.status_word(torch.device("cuda", index))
     return t.data_ptr()
 
 
@@ -154,20 +176,23 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
                 or cs.device != q.device, "cs must be a contiguous fp32 [positions, D / 2, 2] table")
     if not q.is_cuda:
         return paged_append_ref(q, k, v, k_pages, v_pages, block_table, kv_len, cu_q, cs)
-    _strided(k, "k")
-    _strided(v, "v")
-    out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    if not (_aligned(k) and _aligned(v)):
+        _strided(k, "k")
+        _strided(v, "v")
+    out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
     if T == 0:
         return out
-    kp, vp = k_pages.stride(), v_pages.stride()
-    a = _lib.PagedAppendArgs(
+    dev = q.get_device()
+    args = _lib.PAGED_APPEND_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        block_table.data_ptr(), kv_len.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
-        None if cs is None else cs.data_ptr(), _status(q.device),
+        block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+        0 if cs is None else cs.data_ptr(), _status(dev),
         T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], 0 if cs is None else cs.shape[0],
-        block_table.stride(0), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        kp[0], kp[1], kp[2], vp[0], vp[1], vp[2])
-    _launch(_lib.load().lb_paged_append, a, q.device, "lb_paged_append")
+        block_table.stride(0), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3],
+        *v_pages.stride()[:3])
+    with _on(dev):
+        rc = _lib.load().lb_paged_append(args, _lib.stream_ptr())
+    _lib.check(rc, "lb_paged_append")
     return out
 
 
@@ -217,21 +242,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _refuse(not scale >= 0.0, "scale must not be negative")
     if not q.is_cuda:
         return paged_attention_ref(q, k_pages, v_pages, block_table, kv_len, cu_q, scale, window, sinks)
-    out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
     if T == 0:
         return out
-    kp, vp = k_pages.stride(), v_pages.stride()
-    a = _lib.PagedAttnArgs(
+    dev = q.get_device()
+    args = _lib.PAGED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
-        None if cu_q is None else cu_q.data_ptr(), _status(q.device),
+        0 if cu_q is None else cu_q.data_ptr(), _status(dev),
         T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, max_q, scale,
-        block_table.stride(0), q.stride(0), q.stride(1), kp[0], kp[1], kp[2], vp[0], vp[1], vp[2])
+        block_table.stride(0), *q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
     lib = _lib.load()
-    with _on(q.device):
-        need = lib.lb_paged_attention_workspace(C.byref(a))
+    with _on(dev):
+        need = lib.lb_paged_attention_workspace(args)
         # a buffer of this call alone, from the allocator of the current stream (or graph)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        rc = lib.lb_paged_attention(C.byref(a), None if ws is None else ws.data_ptr(), _lib.stream_ptr())
+        rc = lib.lb_paged_attention(args, None if ws is None else ws.data_ptr(), _lib.stream_ptr())
     _lib.check(rc, "lb_paged_attention")
     return out
 
@@ -270,8 +295,8 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
         src, dst = src.to(pool.device), dst.to(pool.device)
     _refuse(src.device != pool.device, "page ids must be on the pool's device or in host memory")
     src, dst = src.contiguous(), dst.contiguous()
-    with _on(pool.device):
+    with _on(pool.get_device()):
         rc = _lib.load().lb_copy_pages(pool.data_ptr(), pool.stride(0) * es, pool.stride(1) * es, page_bytes, rows, n_pages,
-                                       src.data_ptr(), dst.data_ptr(), n, _status(pool.device), _lib.stream_ptr())
+                                       src.data_ptr(), dst.data_ptr(), n, _status(pool.get_device()), _lib.stream_ptr())
     _lib.check(rc, "lb_copy_pages")
     return pool
