@@ -27,7 +27,7 @@ from .config import dump_config
 from .data.pipeline import init_choice_state, setup_sources
 from .distributed import (DistributedArgs, dist_mean_dict, get_global_rank, get_world_size,
                           setup_torch_distributed)
-from .generation import (PackedCausalTransformerGenerator, PackedCausalTransformerGeneratorArgs,
+from .generation import (PackedCausalTransformerGeneratorArgs, build_generator,
                          load_consolidated_model_and_tokenizer)
 
 EVAL_FOLDER_NAME = "{:010d}"
@@ -186,7 +186,7 @@ def eval_on_val(generator, val_args: ValidationArgs, train_cfg: dict):
     return all_metrics
 
 
-def launch_eval(cfg: EvalArgs, generator_cls=PackedCausalTransformerGenerator, model_cls=None, model_args_cls=None,
+def launch_eval(cfg: EvalArgs, generator_cls=build_generator, model_cls=None, model_args_cls=None,
                 loader=None):
     """``loader(consolidated_dir) -> (model, tokenizer, train config)`` replaces the default checkpoint loader."""
     if not dist.is_initialized():
@@ -211,6 +211,8 @@ def launch_eval(cfg: EvalArgs, generator_cls=PackedCausalTransformerGenerator, m
     else:
         model, tokenizer, train_cfg = load_consolidated_model_and_tokenizer(str(consolidated), **kw)
     model.eval()
+    if cfg.generator.samples_per_prompt != 1:
+        raise ValueError("evaluation takes one continuation of every prompt")
     generator = generator_cls(cfg.generator, model, tokenizer)
     results = {"results": {}}
     if cfg.harness is not None and cfg.harness.tasks:

@@ -17,7 +17,7 @@ import math
 import time
 from dataclasses import dataclass, field
 from pathlib import Path
-from typing import List, Optional
+from typing import Dict, List, Optional
 
 import torch
 import torch.nn as nn
@@ -28,6 +28,7 @@ from .config import dataclass_from_dict, load_yaml
 from .models.transformer import Attention, LMTransformer, LMTransformerArgs
 from .ops import _lib
 from .ops.attention import flash_fwd
+from .ops.logits import penalize_logits
 from .tokenizer import Tokenizer, build_tokenizer
 
 
@@ -110,6 +111,8 @@ class CachePlan:
 
 
 class KVCache(nn.Module):
+    rotates = False  # native path: gets queries and keys that are rotated already
+
     def __init__(self, max_tokens, n_kv_heads, head_dim, dtype, device, plan: CachePlan):
         super().__init__()
         self.register_buffer("k_cache", torch.zeros(max_tokens, n_kv_heads, head_dim, dtype=dtype, device=device))
@@ -173,10 +176,81 @@ class PackedCausalTransformerGeneratorArgs:
     show_progress: bool = False
     dtype: Optional[str] = "bf16"
     device: Optional[str] = "cuda"
+    # Extension: logits of every sampled token before the sampler sees them (ops/logits.py)
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None  # token id -> added to its logit
+    allowed_tokens: Optional[List[int]] = None  # nothing else is sampled
+    # Extension: paged KV cache (generation_paged.py); 0 = the contiguous cache
+    page_size: int = 0
+    prefill_chunk: Optional[int] = None  # prompt tokens per forward pass
+    samples_per_prompt: int = 1
+    attention_window: Optional[int] = None  # default: the model's sliding window
+    attention_sinks: int = 0  # first tokens that stay visible behind the window
+
+
+class LogitControls:
+    """Penalties, biases and masks of a generation batch; keeps the token history they need on the device.
+
+    ``grammar``: callable of the generated token lists that returns the tokens allowed next as a bit mask (int32
+    [n_seqs, ceil(vocab / 32)], see ``ops.logits.penalize_logits``), or None."""
+
+    def __init__(self, cfg: PackedCausalTransformerGeneratorArgs, grammar=None):
+        self.repetition, self.presence, self.frequency = cfg.repetition_penalty, cfg.presence_penalty, cfg.frequency_penalty
+        self.bias_of, self.allowed_ids, self.grammar = cfg.logit_bias, cfg.allowed_tokens, grammar
+
+    def __bool__(self):
+        return (self.repetition != 1.0 or self.presence != 0.0 or self.frequency != 0.0 or bool(self.bias_of)
+                or self.allowed_ids is not None or self.grammar is not None)
+
+    def start(self, prompts: List[List[int]], room: int, device):
+        width = max(len(p) for p in prompts)
+        rows = torch.zeros(len(prompts), width + room, dtype=torch.long)
+        for i, p in enumerate(prompts):
+            rows[i, :len(p)] = torch.tensor(p, dtype=torch.long)
+        self.history = rows.to(device)
+        self.prompt_len = torch.tensor([len(p) for p in prompts], dtype=torch.int32).to(device)
+        self.length = self.prompt_len.clone()
+        self.bias = self.allowed = None
+
+    def apply(self, logits: torch.Tensor, generated: List[List[int]]) -> torch.Tensor:
+        """logits [n_seqs, vocab] -> what is sampled from."""
+        V, dev = logits.shape[1], logits.device
+        if self.bias_of and self.bias is None:
+            self.bias = torch.zeros(V, device=dev)
+            for t, b in self.bias_of.items():
+                self.bias[int(t)] = float(b)
+        if self.allowed_ids is not None and self.allowed is None:
+            ok = torch.zeros((V + 31) // 32 * 32, dtype=torch.int64)
+            ok[torch.tensor(self.allowed_ids, dtype=torch.long)] = 1
+            words = (ok.view(-1, 32) << torch.arange(32)).sum(1)
+            self.allowed = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int().to(dev).expand(logits.shape[0], -1)
+        allowed = self.allowed
+        if self.grammar is not None:
+            mask = self.grammar(generated)
+            if mask is not None:
+                mask = mask.to(dev)
+                allowed = mask if allowed is None else mask & allowed
+        return penalize_logits(logits, self.history, self.length, self.prompt_len, self.repetition, self.presence,
+                               self.frequency, self.bias, allowed)
+
+    def took(self, tokens: torch.Tensor) -> None:
+        """tokens [n_seqs]: what was sampled."""
+        self.history.scatter_(1, self.length.long().unsqueeze(1), tokens.view(-1, 1))
+        self.length += 1
 
 
 class PackedCausalTransformerGenerator:
-    def __init__(self, cfg: PackedCausalTransformerGeneratorArgs, model: nn.Module, tokenizer: Tokenizer):
+    samples = 1  # continuations of every prompt
+
+    def __init__(self, cfg: PackedCausalTransformerGeneratorArgs, model: nn.Module, tokenizer: Tokenizer,
+                 paged: bool = False):
+        if not paged and (cfg.page_size or cfg.prefill_chunk or cfg.samples_per_prompt != 1 or cfg.attention_window
+                          or cfg.attention_sinks):
+            raise ValueError("page_size, prefill_chunk, samples_per_prompt, attention_window and attention_sinks need the "
+                             "paged generator of a transformer (build_generator)")
+        self.controls = LogitControls(cfg)
         self.model, self.tokenizer = model, tokenizer
         self.temperature, self.top_p, self.top_k = cfg.temperature, cfg.top_p, cfg.top_k
         self.max_gen_len, self.max_tokens, self.max_prompt_len = cfg.max_gen_len, cfg.max_tokens, cfg.max_prompt_len
@@ -267,13 +341,25 @@ class PackedCausalTransformerGenerator:
         self._graph.replay()
         return self._g_out
 
+    def cache_need(self, prompt_len: int) -> int:
+        """Cache slots that a prompt and what is generated from it take."""
+        return prompt_len + self.max_gen_len
+
+    def _sample(self, logits: torch.Tensor, generated: List[List[int]]) -> torch.Tensor:
+        """logits [1, n_seqs, vocab] of the next token -> tokens [1, n_seqs]."""
+        if not self.controls:
+            return sample_tokens(logits.clone(), self.temperature, self.top_p, self.top_k)
+        nxt = sample_tokens(self.controls.apply(logits[0], generated).unsqueeze(0), self.temperature, self.top_p, self.top_k)
+        self.controls.took(nxt[0])
+        return nxt
+
     @torch.inference_mode()
     def generate(self, prompts: List[str]):
         prompts = [self.tokenizer.encode(p, add_bos=True, add_eos=False) for p in prompts]
         max_seqlen = getattr(self.model, "max_seqlen", self.max_tokens)
         max_prompt_len = self.max_prompt_len or min(max_seqlen - self.max_gen_len, self.max_tokens - self.max_gen_len)
         prompts = [p[-max_prompt_len:] for p in prompts]
-        padded_lengths = [len(p) + self.max_gen_len for p in prompts]
+        padded_lengths = [self.cache_need(len(p)) for p in prompts]
         generation, loglikelihood, greedy = [], [], []
         batches = batch_prompts(prompts, self.max_tokens, lengths=padded_lengths)
         if self.show_progress:
@@ -281,20 +367,26 @@ class PackedCausalTransformerGenerator:
 
             batches = tqdm(batches)
         for batch in batches:
-            n_seqs = len(batch)
+            n_seqs = len(batch) * self.samples
             generated = [[] for _ in range(n_seqs)]
             is_done = [False] * n_seqs
             packed, lengths = pack_prompts(batch)
             packed, lengths = packed.to(self.device), lengths.to(self.device)
             prompt_logits = self.prefill(packed.unsqueeze(0), lengths)
-            all_tokens = sample_tokens(prompt_logits, self.temperature, self.top_p, self.top_k)
-            start_token = all_tokens[:, lengths.cumsum(0) - 1]
+            if self.controls or self.samples > 1:
+                last = prompt_logits[:, lengths.cumsum(0) - 1].repeat_interleave(self.samples, dim=1)
+                if self.controls:
+                    self.controls.start([p for p in batch for _ in range(self.samples)], self.max_gen_len, last.device)
+                start_token = self._sample(last, generated)
+            else:
+                all_tokens = sample_tokens(prompt_logits, self.temperature, self.top_p, self.top_k)
+                start_token = all_tokens[:, lengths.cumsum(0) - 1]
             for i, tok in enumerate(start_token.squeeze(0).tolist()):
                 generated[i].append(tok)
             current = start_token
             for _ in range(1, self.max_gen_len):
                 logits = self.generate_next_token(current)
-                nxt = sample_tokens(logits.clone(), self.temperature, self.top_p, self.top_k)
+                nxt = self._sample(logits, generated)
                 for i, tok in enumerate(nxt.squeeze(0).tolist()):
                     if not is_done[i]:
                         generated[i].append(tok)
@@ -313,6 +405,15 @@ class PackedCausalTransformerGenerator:
                 greedy.append((x.argmax(dim=-1) == y).cpu())
         self.release_cache()
         return generation, loglikelihood, greedy
+
+
+def build_generator(cfg: PackedCausalTransformerGeneratorArgs, model: nn.Module, tokenizer: Tokenizer):
+    """The generator of a transformer that ``cfg.page_size`` asks for."""
+    if cfg.page_size > 0:
+        from .generation_paged import PagedCausalTransformerGenerator
+
+        return PagedCausalTransformerGenerator(cfg, model, tokenizer)
+    return PackedCausalTransformerGenerator(cfg, model, tokenizer)
 
 
 def load_consolidated_model_and_tokenizer(consolidated_path, model_cls=LMTransformer,
@@ -342,7 +443,7 @@ def main(argv=None):
     gen_cfg = dataclass_from_dict(PackedCausalTransformerGeneratorArgs, cfg, strict=False)
     print(cfg)
     model, tokenizer, _ = load_consolidated_model_and_tokenizer(cfg["ckpt"])
-    generator = PackedCausalTransformerGenerator(gen_cfg, model, tokenizer)
+    generator = build_generator(gen_cfg, model, tokenizer)
     prompts = []
     while True:
         prompt = input("Enter a prompt (or press enter to finish): ")
@@ -354,6 +455,6 @@ def main(argv=None):
     dt = time.time() - t0
     total = sum(len(tokenizer.encode(g, False, False)) for g in generation)
     for i, g in enumerate(generation):
-        print(f"\nPrompt {i + 1}: {prompts[i]}")
+        print(f"\nPrompt {i // generator.samples + 1}: {prompts[i // generator.samples]}")
         print(f"Generated Text: {g}")
     print(f"\nTokens per second: {total / dt:.2f}")

@@ -24,7 +24,7 @@ import torch.nn.functional as TF
 from .checkpoint import CONSOLIDATE_NAME
 from .config import dataclass_from_dict, load_yaml
 from .data.regex_cutting import RegexArgs, RegexPool
-from .generation import (CachePlan, KVCache, PackedCausalTransformerGeneratorArgs, batch_prompts, sample_tokens)
+from .generation import (CachePlan, KVCache, LogitControls, PackedCausalTransformerGeneratorArgs, batch_prompts, sample_tokens)
 from .models.aunet import HierarchicalArgs, HierarchicalTransformer, make_level_plan
 from .models.transformer import Attention, RotaryEmbedding
 from .tokenizer import build_tokenizer
@@ -81,6 +81,9 @@ class PackedHierarchicalCausalTransformerGenerator:
 
     def __init__(self, cfg: PackedHierarchicalCausalTransformerGeneratorArgs, model: HierarchicalTransformer, tokenizer,
                  regex_pool: RegexPool):
+        if LogitControls(cfg) or cfg.page_size or cfg.prefill_chunk or cfg.samples_per_prompt != 1 or cfg.attention_window \
+                or cfg.attention_sinks:
+            raise ValueError("the byte model's generator has neither logit controls nor a paged cache")
         self.model, self.tokenizer, self.regex_pool = model, tokenizer, regex_pool
         self.temperature, self.top_p, self.top_k = cfg.temperature, cfg.top_p, cfg.top_k
         self.max_gen_len, self.max_tokens, self.max_prompt_len = cfg.max_gen_len, cfg.max_tokens, cfg.max_prompt_len

@@ -323,10 +323,13 @@ class TransformerBlock(nn.Module):
                                           *at.qkv_weights())
         x = x if h is None else h
         if at.kv_cache is not None:  # generation: rotate, then attend through the KV cache
-            F.rope_(qkv, cs, at.n_heads + at.n_kv_heads, at.head_dim, S, pos)
             t = qkv.view(B * S, at.n_heads + 2 * at.n_kv_heads, at.head_dim)
-            o = at.kv_cache.native_attention(t[:, :at.n_heads], t[:, at.n_heads:at.n_heads + at.n_kv_heads],
-                                             t[:, at.n_heads + at.n_kv_heads:])
+            q, k, v = t.split((at.n_heads, at.n_kv_heads, at.n_kv_heads), dim=1)
+            if at.kv_cache.rotates:
+                o = at.kv_cache.native_attention(q, k, v, cs)
+            else:
+                F.rope_(qkv, cs, at.n_heads + at.n_kv_heads, at.head_dim, S, pos)
+                o = at.kv_cache.native_attention(q, k, v)
         else:
             o = fused.RopeAttnFn.apply(qkv, cs, B, S, at.n_heads, at.n_kv_heads, at.head_dim, causal, doc_start,
                                        doc_end, window, pos, at.wo.weight)

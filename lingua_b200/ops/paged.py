@@ -290,7 +290,6 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
     _refuse(not pool[0, 0].is_contiguous() or page_bytes % 16 or pool.data_ptr() % 16
             or any(k > 1 and (s * es % 16 or s <= 0) for k, s in zip((rows, n_pages), pool.stride()[:2])),
             "a page must be contiguous, a multiple of 16 bytes and 16-byte aligned")
-    _refuse(rows > 65535, "too many rows")
     if not src.is_cuda:
         src, dst = src.to(pool.device), dst.to(pool.device)
     _refuse(src.device != pool.device, "page ids must be on the pool's device or in host memory")
