@@ -5,8 +5,8 @@
 //     -> x + bias,  -inf where the row's bit mask has a zero
 //
 // Bound by the logits' bytes (read and written once). One block per (piece of the vocabulary, row). Every thread first
-// issues the loads of its part of the piece; while they are on their way the block counts the occurrences of the piece's
-// tokens in the row's history, in shared memory, by integer atomics (their order does not matter). The history is read
+// issues the loads of its part of the piece and of the history; then the block counts the occurrences of the piece's
+// tokens in the history, in shared memory, by integer atomics (their order does not matter). The history is read
 // once per piece, from L2, so a piece is as large as shared memory for eight blocks on an SM allows.
 #include "common.cuh"
 #include "lingua_b200.h"
@@ -15,6 +15,7 @@ namespace lb {
 
 constexpr int LG_THREADS = 256;
 constexpr int LG_VECS = 4;  // 16-byte vectors of a thread
+constexpr int LG_HIST = 8;  // history entries of a thread that are requested together with the logits
 
 template <typename T> struct LgVec;
 template <> struct LgVec<float> {
@@ -43,7 +44,7 @@ template <> struct LgVec<__nv_bfloat16> {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(LG_THREADS) penalize_kernel(const LbPenalizeArgs a) {
+__global__ void __launch_bounds__(LG_THREADS, 4) penalize_kernel(const LbPenalizeArgs a) {
   using Vec = LgVec<T>;
   constexpr int PIECE = LG_THREADS * LG_VECS * Vec::N;
   __shared__ __align__(16) int cnt[PIECE];  // low 31 bits: generated occurrences; sign bit: seen at all
@@ -60,19 +61,30 @@ __global__ void __launch_bounds__(LG_THREADS) penalize_kernel(const LbPenalizeAr
     const int i = u * LG_THREADS + threadIdx.x;
     if (i < n_vec) x[u] = reinterpret_cast<const uint4*>(in)[i];
   }
+  const long long* hist = a.history + row * a.history_stride;
+  long long id[LG_HIST];
+#pragma unroll
+  for (int u = 0; u < LG_HIST; ++u) {
+    const int i = u * LG_THREADS + threadIdx.x;
+    if (i < a.L) id[u] = __ldg(hist + i);
+  }
   for (int i = threadIdx.x; i < (n + 3) / 4; i += LG_THREADS) reinterpret_cast<int4*>(cnt)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   const int total = max(0, min(a.history_len[row], a.L));
   const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
-  const long long* hist = a.history + row * a.history_stride;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < total; i += LG_THREADS) {
-    const long long t = hist[i] - v0;
+  auto count = [&](int i, long long token) {
+    const long long t = token - v0;
     if (t >= 0 && t < n) {
       atomicOr(&cnt[t], (int)0x80000000);
       if (i >= prompt) atomicAdd(&cnt[t], 1);
     }
+  };
+#pragma unroll
+  for (int u = 0; u < LG_HIST; ++u) {
+    const int i = u * LG_THREADS + threadIdx.x;
+    if (i < total) count(i, id[u]);
   }
+  for (int i = LG_HIST * LG_THREADS + threadIdx.x; i < total; i += LG_THREADS) count(i, hist[i]);
   const float rep = a.repetition ? a.repetition[row] : a.repetition_s;
   const float pres = a.presence ? a.presence[row] : a.presence_s;
   const float freq = a.frequency ? a.frequency[row] : a.frequency_s;

@@ -15,10 +15,9 @@ namespace lb {
 // and arrive while it runs. 24 prompts, 5300 tokens of 48 heads (64 MB): see the table of measurements.
 constexpr int AP_HEADS = 8;
 __global__ void __launch_bounds__(128) paged_append_kernel(const LbPagedAppendArgs a) {
-  const int vph = a.D / 8;
-  const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-  if (i >= (long long)a.T * vph) return;
-  const int tok = (int)(i / vph), v = (int)(i % vph);
+  const int vph = a.D / 8, v = threadIdx.x & (vph - 1);  // 8 or 16 vectors of a head
+  const int tok = blockIdx.x * (128 / vph) + threadIdx.x / vph;
+  if (tok >= a.T) return;
   const int h0 = blockIdx.y * AP_HEADS, n_heads = min(AP_HEADS, a.H + 2 * a.Hkv - h0);
   uint4 x[AP_HEADS];
 #pragma unroll
@@ -45,18 +44,19 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const LbPagedAppendAr
     at = tok - c0;
     if (tok < c0 || tok >= c1) seq = -1;  // a padding row
   }
+  const int page_log = __ffs(a.page) - 1;
   long long pos = -1;
   if (seq >= 0) pos = (long long)a.kv_len[seq] - n_new + at;
   __nv_bfloat16 *kd = nullptr, *vd = nullptr;
   float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
   if (pos >= 0) {
-    const long long col = pos / a.page;
+    const int col = (int)min(pos >> page_log, 0x7FFFFFFFll);
     const int page = col < a.cols ? a.table[seq * a.table_stride + col] : -1;
     if (page < 0 || page >= a.n_pages || (a.cs && pos >= a.cs_rows)) {
       if (a.status) atomicOr(a.status, ST_BAD_ARG | 0x41u);
       pos = -1;
     } else {
-      const long long row = pos % a.page;
+      const int row = (int)pos & (a.page - 1);
       kd = (__nv_bfloat16*)a.k_pages + page * a.kp_sp + row * a.kp_st + v * 8;
       vd = (__nv_bfloat16*)a.v_pages + page * a.vp_sp + row * a.vp_st + v * 8;
       if (a.cs) {
@@ -124,10 +124,10 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(char* pool, long long s
 extern "C" int lb_paged_append(const LbPagedAppendArgs* a, void* stream) {
   using namespace lb;
   if (a->D != 64 && a->D != 128) return 1;
-  if (a->H <= 0 || a->Hkv <= 0 || a->page <= 0) return 2;
+  if (a->H <= 0 || a->Hkv <= 0 || a->page <= 0 || (a->page & (a->page - 1))) return 2;
   if (a->T <= 0) return 0;
-  const long long threads = (long long)a->T * (a->D / 8);
-  const dim3 grid((unsigned)((threads + 127) / 128), (a->H + 2 * a->Hkv + AP_HEADS - 1) / AP_HEADS);
+  const int toks = 128 / (a->D / 8);
+  const dim3 grid((a->T + toks - 1) / toks, (a->H + 2 * a->Hkv + AP_HEADS - 1) / AP_HEADS);
   paged_append_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(*a);
   g_launches.fetch_add(1, std::memory_order_relaxed);
   const cudaError_t e = cudaGetLastError();
