@@ -5,8 +5,10 @@
 //
 // Bound by reading every visible key and value row once (2 D 2 bytes per key and kv head; G = H / Hkv query heads share
 // them). Layout of the work:
-//  * An item is (sequence, kv head, 16 rows), the rows being (token, head of the group) pairs, so that one pass over the
-//    keys serves the whole group on m16n8k16 tensor-core products (16 x 8 keys of scores, then 16 rows x 8 channels).
+//  * An item is (sequence, kv head, 8 or 16 rows), the rows being (token, head of the group) pairs, so that one pass over
+//    the keys serves the whole group. The products are m16n8k16 with the KEYS on the 16 side and the rows on the 8 side,
+//    S^T = K Q^T and O^T = V^T P^T: with the rows on the 16 side, as one would write them first, one token of up to 8
+//    heads would fill half of every product.
 //  * The key axis of an item is cut into blocks of 64 keys. All blocks of all items, in order, are dealt out in equal
 //    contiguous shares to the blocks of a fixed grid, so a batch of any mix of lengths keeps every SM equally busy; an
 //    item that crosses a share boundary leaves partial results (running maximum, sum, unnormalised output, fp32) that
@@ -16,12 +18,10 @@
 //  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. Every warp
 //    keeps its own ring of 16-key stages in shared memory, filled by TMA (boxes of 16 keys x 64 channels, 128-byte
 //    swizzle), so a stage is waited for and given back by one warp alone.
-//  * A lane reads 16-byte pieces and feeds them to the products as they are. That permutes the contraction index (the
-//    same way for q and k), the keys of an 8-key tile and the output channels; none of it changes a result. Column n of a
-//    tile is key sw(n) = (n >> 1) | (n & 1) << 2, and likewise lane row n takes the channel piece sw(n) of the values: with
-//    the swizzle, the eight lanes of a quarter warp then read eight different 16-byte columns of banks.
+//  * ldmatrix reads both operands in place, the values transposed; the swizzle makes its eight rows fall into different
+//    banks. P^T is turned from the layout of a result to that of an operand by movmatrix.
 //  * Keys that no row may see, and pages that are not there, never contribute: scores are replaced (not added to), and
-//    value pieces of hidden keys are zeroed in registers, so what a page holds past the end of a sequence (NaN included)
+//    values of hidden keys are zeroed in registers, so what a page holds past the end of a sequence (NaN included)
 //    or behind the window does not matter.
 #include <algorithm>
 #include "common.cuh"
@@ -30,33 +30,39 @@
 namespace lb {
 
 constexpr int DEC_BLOCK = 64;       // keys per block: 16 for each warp
-constexpr int DEC_ROWS = 16;
 constexpr int NOSPLIT_BLOCKS = 8;
 constexpr int MIN_SHARE = 2;
 constexpr float DEC_LOG2E = 1.4426950408889634f;
 
-template <int D>
+template <int D, int NT>
 struct DecCfg {
-  static constexpr int KI = D / 32;            // 16-byte pieces of a key row that a lane takes
+  static constexpr int ROWS = 8 * NT;
   static constexpr int VG = D / 64;            // 64-channel boxes of a row
   static constexpr int BOX = 16 * 128;         // 16 keys x 64 channels
   static constexpr int STAGE = 2 * VG * BOX;   // bytes of one warp's stage: key boxes, then value boxes
   static constexpr int NST = D == 128 ? 3 : 6;
   static constexpr int SMEM = 4 * NST * STAGE + 1024;  // 97 KB: two blocks per SM
   static constexpr int OROW = D + 4;                // padded row of the merge buffer (floats)
-  static constexpr int SLOT = DEC_ROWS * D + 2 * DEC_ROWS;  // floats of one partial result
+  static constexpr int SLOT = ROWS * D + 2 * ROWS;  // floats of one partial result
 };
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&m)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&m)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // What a sequence asks for.
@@ -67,9 +73,10 @@ struct DecSeq {
   int wlo;          // first key inside some row's window
   int sb, wb;       // 64-key blocks: [0, sb) for the first tokens, then from wb on
   int nb;           // blocks of an item (at least one: rows that see nothing still get their zeros)
-  int rt;           // 16-row tiles
+  int rt;           // row tiles
 };
 
+template <int ROWS>
 __device__ __forceinline__ DecSeq dec_seq(const LbPagedAttnArgs& a, int s, bool report) {
   DecSeq r;
   r.q0 = a.cu_q ? a.cu_q[s] : s;
@@ -89,7 +96,7 @@ __device__ __forceinline__ DecSeq dec_seq(const LbPagedAttnArgs& a, int s, bool 
   r.sb = min((min(a.sinks, r.wlo) + DEC_BLOCK - 1) / DEC_BLOCK, r.wb);
   r.nb = max(1, r.sb + (r.end + DEC_BLOCK - 1) / DEC_BLOCK - r.wb);
   const long long rows = (long long)r.nq * (a.H / a.Hkv);
-  r.rt = (int)((rows + DEC_ROWS - 1) / DEC_ROWS);
+  r.rt = (int)((rows + ROWS - 1) / ROWS);
   return r;
 }
 
@@ -101,17 +108,18 @@ struct DecWork {  // found by one thread, read by the block
 
 // Workspace: per block two partial results (its first item when an earlier block began it, its last item when a later
 // block ends it) and one int4 header naming the item it began without ending: (sequence, kv head, row tile, parts).
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_constant__ CUtensorMap tk,
                                                               const __grid_constant__ CUtensorMap tv,
                                                               const LbPagedAttnArgs a, float* ws, int4* hdr) {
-  using Cfg = DecCfg<D>;
+  using Cfg = DecCfg<D, NT>;
+  constexpr int ROWS = Cfg::ROWS;
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[4][Cfg::NST];
   __shared__ int abort_flag;
   __shared__ long long warp_sum[4];
   __shared__ DecWork work;
-  __shared__ float sm_m[4][DEC_ROWS], sm_l[4][DEC_ROWS];
+  __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int G = a.H / a.Hkv;
@@ -132,7 +140,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   const int s_lo = min(a.n_seqs, (int)threadIdx.x * per), s_hi = min(a.n_seqs, s_lo + per);
   long long mine = 0;
   for (int s = s_lo; s < s_hi; ++s) {
-    const DecSeq q = dec_seq(a, s, blockIdx.x == 0);
+    const DecSeq q = dec_seq<ROWS>(a, s, blockIdx.x == 0);
     mine += (long long)a.Hkv * q.rt * (split ? q.nb : 1);
   }
   long long incl = mine;
@@ -157,7 +165,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   if (u0 < u1 && u0 >= before && u0 < before + mine) {
     long long at = before;
     for (int s = s_lo; s < s_hi; ++s) {
-      const DecSeq q = dec_seq(a, s, false);
+      const DecSeq q = dec_seq<ROWS>(a, s, false);
       const long long n = (long long)a.Hkv * q.rt * (split ? q.nb : 1);
       if (u0 < at + n) { work.first = u0; work.last = u1; work.seq = s; work.offset = u0 - at; break; }
       at += n;
@@ -182,14 +190,22 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   uint32_t parity = 0;  // bit st: phase the next wait on stage st completes
   int head = 0;         // stage of the next block to be read
   bool alive = true;
-  const int sr = (r >> 1) | ((r & 1) << 2);  // sw(r)
+  // ldmatrix row of this lane: matrix lane >> 3, row lane & 7. Keys: matrices (keys 0-7, piece), (keys 8-15, piece), then the
+  // next piece; values: (keys 0-7, piece), (keys 0-7, next piece), then keys 8-15. Offsets of pieces 2 p, 2 p + 1 of a box.
+  const int k_row = (lane & 7) + 8 * ((lane >> 3) & 1), v_row = (lane & 7) + 8 * (lane >> 4);
+  uint32_t k_off[4], v_off[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    k_off[p] = k_row * 128 + (((2 * p + (lane >> 4)) ^ (lane & 7)) << 4);
+    v_off[p] = v_row * 128 + (((2 * p + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+  }
   const float sl2 = a.scale * DEC_LOG2E;
   const int page_log = __ffs(a.page) - 1;
   long long left = u1 - u0;
   int seq = work.seq;
   long long offset = work.offset;
   for (; left > 0 && seq < a.n_seqs; ++seq, offset = 0) {
-    const DecSeq q = dec_seq(a, seq, false);
+    const DecSeq q = dec_seq<ROWS>(a, seq, false);
     const int item_units = split ? q.nb : 1;
     const long long n_items = (long long)a.Hkv * q.rt;
     for (long long item = offset / item_units; left > 0 && item < n_items; ++item) {
@@ -198,21 +214,25 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
       const int b1 = split ? (int)min((long long)q.nb, b0 + left) : q.nb;
       left -= split ? b1 - b0 : 1;
 
-      // ---- q fragments: lane (r, c) holds channels 32 i + 8 c .. + 7 of rows r and r + 8
-      const int row0 = rt * DEC_ROWS;
-      const int n_rows = min(DEC_ROWS, q.nq * G - row0);
-      uint4 qf[Cfg::KI][2];
-      long long pos[2];
+      // ---- Q^T fragments: lane (r, c) holds channels 16 k + 2 c, + 1, + 8, + 9 of row 8 t + r
+      const int row0 = rt * ROWS;
+      const int n_rows = min(ROWS, q.nq * G - row0);
+      uint32_t qf[D / 16][NT][2];
+      long long pos[NT][2];  // of rows 8 t + 2 c, + 1
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int row = row0 + r + 8 * hf;
-        const bool live = r + 8 * hf < n_rows;
-        pos[hf] = live ? q.pos0 + row / G : -1;
+      for (int t = 0; t < NT; ++t) {
+        const int row = row0 + 8 * t + r;
+        const bool live = 8 * t + r < n_rows;
         const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (long long)(q.q0 + row / G) * a.q_st +
-                                  (long long)(hk * G + row % G) * a.q_sh + 8 * c;
+                                  (long long)(hk * G + row % G) * a.q_sh + 2 * c;
 #pragma unroll
-        for (int i = 0; i < Cfg::KI; ++i)
-          qf[i][hf] = live ? *reinterpret_cast<const uint4*>(qp + 32 * i) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][t][0] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
+          qf[k][t][1] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          pos[t][i] = 8 * t + 2 * c + i < n_rows ? q.pos0 + (row0 + 8 * t + 2 * c + i) / G : -1;
       }
 
       // ---- pages of this warp's next 32 + 32 blocks, one per lane
@@ -245,14 +265,18 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         }
       };
 
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-      float acc[Cfg::VG][8][4];
+      // rows 8 t + 2 c + i: maximum, sum, and O^T: acc[j][t][2 h + i] is channel 16 j + 8 h + r
+      float m[NT][2], l[NT][2];
+      float acc[D / 16][NT][4];
 #pragma unroll
-      for (int g = 0; g < Cfg::VG; ++g)
+      for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int i = 0; i < 2; ++i) { m[t][i] = -INFINITY; l[t][i] = 0.f; }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[g][e][i] = 0.f;
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][t][i] = 0.f;
+      }
 
       auto next = [](int st) { return st + 1 == Cfg::NST ? 0 : st + 1; };
       int fill = head;
@@ -266,102 +290,85 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         if (!alive) break;
         parity ^= 1u << head;
         const uint32_t kbox = ring + head * Cfg::STAGE, vbox = kbox + Cfg::VG * Cfg::BOX;
-        uint4 kf[2][Cfg::KI], vf[4][Cfg::VG];
-        // key sw(r) + 8 t: its row is row & 7 == sw(r) of the swizzle pattern, pieces 4 (i & 1) + c of box i >> 1
+        // scores: two accumulators for each row tile, so that chains of dependent products are half as long
+        float s[NT][4], s2[NT][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < Cfg::KI; ++i)
-            kf[t][i] = lds128(kbox + (i >> 1) * Cfg::BOX + (sr + 8 * t) * 128 + (((4 * (i & 1) + c) ^ sr) << 4));
-        // keys c, c + 4, c + 8, c + 12; channel piece sw(r)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int g = 0; g < Cfg::VG; ++g)
-            vf[t][g] = lds128(vbox + g * Cfg::BOX + (c + 4 * t) * 128 + ((sr ^ ((c + 4 * t) & 7)) << 4));
-        // two accumulators for each 8 keys: chains of dependent products half as long
-        float s[2][4], s2[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][i] = s2[t][i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < Cfg::KI; ++i) {
-            const uint4 k = kf[t][i];
-            mma16816(s[t], qf[i][0].x, qf[i][1].x, qf[i][0].y, qf[i][1].y, k.x, k.y);
-            mma16816(s2[t], qf[i][0].z, qf[i][1].z, qf[i][0].w, qf[i][1].w, k.z, k.w);
-          }
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t kf[4];
+          ldmatrix_x4(kf, kbox + (k >> 2) * Cfg::BOX + k_off[k & 3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816(k & 1 ? s2[t] : s[t], kf, qf[k][t][0], qf[k][t][1]);
         }
-        // scores in units of log 2; s[t][2 hf + i]: row r + 8 hf, key kb + 8 t + sw(2 c + i) = kb + 8 t + c + 4 i
+        // in units of log 2; s[t][2 h + i]: key kb + r + 8 h, row 8 t + 2 c + i
         const int kb = key_of(b);
         const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
+        bool grow = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             s[t][x] = (s[t][x] + s2[t][x]) * sl2;
             if (!whole) {
-              const int j = kb + 8 * t + c + 4 * (x & 1);
-              const long long p = pos[x >> 1];
+              const int j = kb + r + 8 * (x >> 1);
+              const long long p = pos[t][x & 1];
               if (j > p || j >= q.end || (a.window > 0 && j <= p - a.window && j >= a.sinks)) s[t][x] = -INFINITY;
             }
           }
-        // the running maximum only moves when it would be exceeded by more than 2^8 (probabilities stay below 2^8)
-        float mx[2];
-        bool grow = false;
+          // the running maximum only moves when it would be exceeded by more than 2^8 (probabilities stay below 2^8)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          mx[hf] = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
-          grow |= mx[hf] > m[hf] + 8.f;
+          for (int i = 0; i < 2; ++i) grow |= fmaxf(s[t][i], s[t][2 + i]) > m[t][i] + 8.f;
         }
         if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xFFFFFFFFu, mx[hf], 1));
-            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xFFFFFFFFu, mx[hf], 2));
-            if (mx[hf] > m[hf]) {
-              const float f = m[hf] == -INFINITY ? 0.f : exp2f(m[hf] - mx[hf]);
-              m[hf] = mx[hf];
-              l[hf] *= f;
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int g = 0; g < Cfg::VG; ++g)
+            for (int i = 0; i < 2; ++i) {
+              float mx = fmaxf(s[t][i], s[t][2 + i]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { acc[g][e][2 * hf] *= f; acc[g][e][2 * hf + 1] *= f; }
+              for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+              if (mx > m[t][i]) {
+                const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - mx);
+                m[t][i] = mx;
+                l[t][i] *= f;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) { acc[j][t][i] *= f; acc[j][t][2 + i] *= f; }
+              }
             }
-          }
         }
         // probabilities enter the second product in bf16 (half a step, 2^-8 of each); their sum is taken before that
-        uint32_t pa[2][2];
+        uint32_t pt[NT][2];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const float mm = m[hf] == -INFINITY ? 0.f : m[hf];
+        for (int t = 0; t < NT; ++t) {
+          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const float p0 = exp2f(s[t][2 * hf] - mm), p1 = exp2f(s[t][2 * hf + 1] - mm);
-            l[hf] += p0 + p1;
-            pa[t][hf] = pack_bf16(p0, p1);
+          for (int h = 0; h < 2; ++h) {
+            const float p0 = exp2f(s[t][2 * h] - m0), p1 = exp2f(s[t][2 * h + 1] - m1);
+            l[t][0] += p0;
+            l[t][1] += p1;
+            pt[t][h] = movmatrix_trans(pack_bf16(p0, p1));
           }
         }
+        uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // keys kb + 2 c, + 1 and those 8 further: which are not hidden
         if (!whole) {
+          keep0 = keep1 = 0;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int j = kb + c + 4 * t;
-            if (j >= q.end || (j < q.wlo && j >= a.sinks))
-#pragma unroll
-              for (int g = 0; g < Cfg::VG; ++g) vf[t][g] = make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 4; ++i) {
+            const int j = kb + 2 * c + (i & 1) + 8 * (i >> 1);
+            const uint32_t bits = j < q.end && (j >= q.wlo || j < a.sinks) ? 0xFFFFu << (16 * (i & 1)) : 0u;
+            if (i < 2) keep0 |= bits; else keep1 |= bits;
           }
         }
 #pragma unroll
-        for (int g = 0; g < Cfg::VG; ++g) {
-          uint32_t v[4][4];
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t vf[4];
+          ldmatrix_x4_trans(vf, vbox + (j >> 2) * Cfg::BOX + v_off[j & 3]);
+          if (!whole) { vf[0] &= keep0; vf[1] &= keep0; vf[2] &= keep1; vf[3] &= keep1; }
 #pragma unroll
-          for (int t = 0; t < 4; ++t) { v[t][0] = vf[t][g].x; v[t][1] = vf[t][g].y; v[t][2] = vf[t][g].z; v[t][3] = vf[t][g].w; }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-            mma16816(acc[g][e], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(v[0][e >> 1], v[1][e >> 1], sel),
-                     __byte_perm(v[2][e >> 1], v[3][e >> 1], sel));
-          }
+          for (int t = 0; t < NT; ++t) mma16816(acc[j][t], vf, pt[t][0], pt[t][1]);
         }
         // every lane's pieces are in registers (the products needed them): the stage can be filled again
         __syncwarp();
@@ -376,32 +383,32 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
 
       // ---- join the four warps
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        l[hf] += __shfl_xor_sync(0xFFFFFFFFu, l[hf], 1);
-        l[hf] += __shfl_xor_sync(0xFFFFFFFFu, l[hf], 2);
-        if (c == 0) { sm_m[warp][r + 8 * hf] = m[hf]; sm_l[warp][r + 8 * hf] = l[hf]; }
-      }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], o);
+          if (r == 0) { sm_m[warp][8 * t + 2 * c + i] = m[t][i]; sm_l[warp][8 * t + 2 * c + i] = l[t][i]; }
+        }
       __syncthreads();
       if (abort_flag) return;  // read by all after the same barrier
       float* obuf = reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)));
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int row = r + 8 * hf;
-        if (row < n_rows) {
-          const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
-          const float f = m[hf] == -INFINITY ? 0.f : exp2f(m[hf] - M);
-          float* dst = obuf + (warp * DEC_ROWS + row) * Cfg::OROW;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int g = 0; g < Cfg::VG; ++g)
+        for (int i = 0; i < 2; ++i) {
+          const int row = 8 * t + 2 * c + i;
+          if (row < n_rows) {
+            const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+            const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - M);
+            float* dst = obuf + (warp * ROWS + row) * Cfg::OROW + r;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int e = 0; e < 8; e += 4)
-                *reinterpret_cast<float4*>(dst + 64 * g + 32 * i + 8 * c + e) =  // pieces sw(2 c + i) = c + 4 i
-                    make_float4(acc[g][e][2 * hf + i] * f, acc[g][e + 1][2 * hf + i] * f, acc[g][e + 2][2 * hf + i] * f,
-                                acc[g][e + 3][2 * hf + i] * f);
+            for (int j = 0; j < D / 16; ++j) {
+              dst[16 * j] = acc[j][t][i] * f;
+              dst[16 * j + 8] = acc[j][t][2 + i] * f;
+            }
+          }
         }
-      }
       __syncthreads();
       const bool whole_item = b0 == 0 && b1 == q.nb;
       float* slot = whole_item ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         float L = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(obuf + (w * DEC_ROWS + row) * Cfg::OROW + ch);
+          const float4 x = *reinterpret_cast<const float4*>(obuf + (w * ROWS + row) * Cfg::OROW + ch);
           o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
           L += sm_m[w][row] == -INFINITY ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);
         }
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
           *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
         } else {
           *reinterpret_cast<float4*>(slot + row * D + ch) = o;
-          if (ch == 0) { slot[DEC_ROWS * D + row] = M; slot[DEC_ROWS * D + DEC_ROWS + row] = L; }
+          if (ch == 0) { slot[ROWS * D + row] = M; slot[ROWS * D + ROWS + row] = L; }
         }
       }
       if (!whole_item && b0 == 0 && threadIdx.x == 0) {
@@ -443,17 +450,18 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
 
 // Joins the parts of the item that block `blockIdx.x` of the kernel above began and later blocks went on with: warps
 // take parts, lanes channels.
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAttnArgs a, const float* ws, const int4* hdr) {
-  using Cfg = DecCfg<D>;
+  using Cfg = DecCfg<D, NT>;
+  constexpr int ROWS = Cfg::ROWS;
   constexpr int E = D / 32;
   __shared__ float sm_o[8][D], sm_m[8], sm_l[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 h = hdr[blockIdx.x];
   if (h.w == 0) return;
-  const DecSeq q = dec_seq(a, h.x, false);
+  const DecSeq q = dec_seq<ROWS>(a, h.x, false);
   const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = h.z * DEC_ROWS + blockIdx.y;
+  const int row = h.z * ROWS + blockIdx.y;
   if (row >= q.nq * G) return;
   auto slot = [&](int part) { return ws + (long long)(part == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + part)) * Cfg::SLOT; };
   float m = -INFINITY, l = 0.f, o[E];
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAtt
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   for (int part = warp; part < h.w; part += 8) {
     const float* p = slot(part);
-    const float pm = p[DEC_ROWS * D + blockIdx.y], pl = p[DEC_ROWS * D + DEC_ROWS + blockIdx.y];
+    const float pm = p[ROWS * D + blockIdx.y], pl = p[ROWS * D + ROWS + blockIdx.y];
     float x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = p[blockIdx.y * D + lane * E + e];
@@ -491,22 +499,22 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAtt
   }
 }
 
-template <int D>
+template <int D, int NT>
 static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
-  using Cfg = DecCfg<D>;
-  if (ensure_dyn_smem<paged_decode_kernel<D>>(Cfg::SMEM)) return 20;
+  using Cfg = DecCfg<D, NT>;
+  if (ensure_dyn_smem<paged_decode_kernel<D, NT>>(Cfg::SMEM)) return 20;
   const int grid = 2 * num_sms();
   int4* hdr = ws ? reinterpret_cast<int4*>((float*)ws + 2ll * grid * Cfg::SLOT) : nullptr;
   // pools as (channel, row of the page, head, page), read in boxes of 64 channels x 16 rows
   CUtensorMap tk, tv;
   if (make_tmap_4d(&tk, a.k_pages, 2, D, a.page, a.kp_st, a.Hkv, a.kp_sh, a.n_pages, a.kp_sp, 64, 16)) return 10;
   if (make_tmap_4d(&tv, a.v_pages, 2, D, a.page, a.vp_st, a.Hkv, a.vp_sh, a.n_pages, a.vp_sp, 64, 16)) return 11;
-  paged_decode_kernel<D><<<grid, 128, Cfg::SMEM, st>>>(tk, tv, a, (float*)ws, hdr);
+  paged_decode_kernel<D, NT><<<grid, 128, Cfg::SMEM, st>>>(tk, tv, a, (float*)ws, hdr);
   g_launches.fetch_add(1, std::memory_order_relaxed);
   if (ws) {
     // starts while the first kernel's last blocks run, and waits for all of it before it reads
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, a.cu_q ? DEC_ROWS : min(DEC_ROWS, a.H / a.Hkv));
+    cfg.gridDim = dim3(grid, a.cu_q ? Cfg::ROWS : std::min(Cfg::ROWS, a.H / a.Hkv));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -514,7 +522,7 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D>, a, (const float*)ws, (const int4*)hdr) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D, NT>, a, (const float*)ws, (const int4*)hdr) != cudaSuccess) {
       return 400 + (int)cudaGetLastError();
     }
     g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -537,10 +545,14 @@ static bool use_chunk(const LbPagedAttnArgs& a) {
   const int G = a.H / a.Hkv;
   const long long rows = (long long)a.max_q * G;
   if (!a.cu_q || G > 128 || rows <= CHUNK_ROWS) return false;
-  const long long blocks = (long long)a.n_seqs * a.Hkv * ((rows + DEC_ROWS - 1) / DEC_ROWS) *
+  const long long blocks = (long long)a.n_seqs * a.Hkv * ((rows + 15) / 16) *
                            (((long long)a.cols * a.page + DEC_BLOCK - 1) / DEC_BLOCK);
   return blocks > 2ll * num_sms() * FEW_BLOCKS;
 }
+// one row tile of 8 where that holds all rows of a sequence, else of 16
+static bool eight_rows(const LbPagedAttnArgs& a) { return (long long)(a.cu_q ? a.max_q : 1) * (a.H / a.Hkv) <= 8; }
+template <int NT>
+static long long decode_slot(int D) { return D == 128 ? DecCfg<128, NT>::SLOT : DecCfg<64, NT>::SLOT; }
 }  // namespace lb
 
 extern "C" long long lb_paged_attention_workspace(const LbPagedAttnArgs* a) {
@@ -549,7 +561,7 @@ extern "C" long long lb_paged_attention_workspace(const LbPagedAttnArgs* a) {
   long long keys = (long long)a->cols * a->page;  // most keys a row can see
   if (a->window > 0 && !a->cu_q) keys = std::min(keys, (long long)a->window + a->sinks);
   if (keys <= NOSPLIT_BLOCKS * DEC_BLOCK) return 0;
-  const long long slot = a->D == 128 ? DecCfg<128>::SLOT : DecCfg<64>::SLOT;
+  const long long slot = eight_rows(*a) ? decode_slot<1>(a->D) : decode_slot<2>(a->D);
   return 2ll * num_sms() * (2 * slot * 4 + 16);
 }
 
@@ -561,6 +573,8 @@ extern "C" int lb_paged_attention(const LbPagedAttnArgs* a, void* workspace, voi
   if ((long long)a->cols * a->page > (1ll << 30)) return 4;
   if (a->T <= 0) return 0;
   if (use_chunk(*a)) return workspace ? paged_chunk_dispatch(*a, workspace, (cudaStream_t)stream) : 5;
-  return a->D == 128 ? launch_decode<128>(*a, workspace, (cudaStream_t)stream)
-                     : launch_decode<64>(*a, workspace, (cudaStream_t)stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (eight_rows(*a))
+    return a->D == 128 ? launch_decode<128, 1>(*a, workspace, st) : launch_decode<64, 1>(*a, workspace, st);
+  return a->D == 128 ? launch_decode<128, 2>(*a, workspace, st) : launch_decode<64, 2>(*a, workspace, st);
 }
