@@ -390,6 +390,10 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x2) {
   unpack_u2(t, t0, t1);
   return pack_u2(p0 + (t0 << 23), p1 + (t1 << 23));
 }
+// a / b of non-negative numbers: 64-bit division is a long subroutine, and most operands fit 32 bits.
+__device__ __forceinline__ long long div_nonneg(long long a, long long b) {
+  return ((unsigned long long)a | (unsigned long long)b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

@@ -30,8 +30,7 @@
 namespace lb {
 
 constexpr int DEC_BLOCK = 64;       // keys per block: 16 for each warp
-constexpr int NOSPLIT_BLOCKS = 8;
-constexpr int MIN_SHARE = 2;
+constexpr int NOSPLIT_BLOCKS = 4;  // 256 keys: 7.2 us whole, 7.9 us cut up; 511 keys 10.1 / 7.7 us (one sequence, 16 heads)
 constexpr float DEC_LOG2E = 1.4426950408889634f;
 
 template <int D, int NT>
@@ -158,10 +157,11 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
     total += warp_sum[w];
   }
   before += incl - mine;
-  // no share is empty (the join kernel counts on that), and small problems are not cut finer than MIN_SHARE
-  const long long n_blocks = max(1ll, min((long long)gridDim.x, split ? total / MIN_SHARE : total));
+  // no share is empty (the join kernel counts on that)
+  const long long n_blocks = max(1ll, min((long long)gridDim.x, total));
   const bool busy = blockIdx.x < n_blocks;
-  const long long u0 = busy ? total * blockIdx.x / n_blocks : 0, u1 = busy ? total * (blockIdx.x + 1) / n_blocks : 0;
+  auto share = [&](long long i) { return div_nonneg(total * i, n_blocks); };  // first unit of share i
+  const long long u0 = busy ? share(blockIdx.x) : 0, u1 = busy ? share(blockIdx.x + 1) : 0;
   if (u0 < u1 && u0 >= before && u0 < before + mine) {
     long long at = before;
     for (int s = s_lo; s < s_hi; ++s) {
@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
     const DecSeq q = dec_seq<ROWS>(a, seq, false);
     const int item_units = split ? q.nb : 1;
     const long long n_items = (long long)a.Hkv * q.rt;
-    for (long long item = offset / item_units; left > 0 && item < n_items; ++item) {
-      const int hk = (int)(item / q.rt), rt = (int)(item % q.rt);
+    for (long long item = div_nonneg(offset, item_units); left > 0 && item < n_items; ++item) {
+      const int hk = (int)div_nonneg(item, q.rt), rt = (int)(item - (long long)hk * q.rt);
       const int b0 = split ? (int)(offset - item * item_units > 0 ? offset - item * item_units : 0) : 0;
       const int b1 = split ? (int)min((long long)q.nb, b0 + left) : q.nb;
       left -= split ? b1 - b0 : 1;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
       }
 
       auto next = [](int st) { return st + 1 == Cfg::NST ? 0 : st + 1; };
-      int fill = head;
+      int fill = head, prev = head;
       for (int b = b0; b < min(b1, b0 + Cfg::NST); ++b) {
         issue(b, fill);
         fill = next(fill);
@@ -303,6 +303,11 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma16816(k & 1 ? s2[t] : s[t], kf, qf[k][t][0], qf[k][t][1]);
         }
+        // what follows needs time until the scores are there: refill the stage of the previous block, read the values
+        if (b > b0 && b + Cfg::NST - 1 < b1) issue(b + Cfg::NST - 1, prev);
+        uint32_t vf[D / 16][4];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) ldmatrix_x4_trans(vf[j], vbox + (j >> 2) * Cfg::BOX + v_off[j & 3]);
         // in units of log 2; s[t][2 h + i]: key kb + r + 8 h, row 8 t + 2 c + i
         const int kb = key_of(b);
         const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
@@ -364,15 +369,12 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-          uint32_t vf[4];
-          ldmatrix_x4_trans(vf, vbox + (j >> 2) * Cfg::BOX + v_off[j & 3]);
-          if (!whole) { vf[0] &= keep0; vf[1] &= keep0; vf[2] &= keep1; vf[3] &= keep1; }
+          if (!whole) { vf[j][0] &= keep0; vf[j][1] &= keep0; vf[j][2] &= keep1; vf[j][3] &= keep1; }
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(acc[j][t], vf, pt[t][0], pt[t][1]);
+          for (int t = 0; t < NT; ++t) mma16816(acc[j][t], vf[j], pt[t][0], pt[t][1]);
         }
-        // every lane's pieces are in registers (the products needed them): the stage can be filled again
-        __syncwarp();
-        if (b + Cfg::NST < b1) issue(b + Cfg::NST, head);
+        __syncwarp();  // every lane's pieces are in registers (the products needed them): the stage can be filled again
+        prev = head;
         head = next(head);
       }
       // a wait ran out (recorded in the status word): copies in flight land before shared memory is given up
@@ -437,9 +439,9 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         // units [u1 - (b1 - b0), + nb) hold this item: find the block its last unit belongs to
         const long long end_unit = u1 - (b1 - b0) + q.nb - 1;
         // share of unit u: the largest i with total * i / n_blocks <= u
-        long long i = (end_unit * n_blocks) / total;
-        while (i + 1 < n_blocks && total * (i + 1) / n_blocks <= end_unit) ++i;
-        while (i > 0 && total * i / n_blocks > end_unit) --i;
+        long long i = div_nonneg(end_unit * n_blocks, total);
+        while (i + 1 < n_blocks && share(i + 1) <= end_unit) ++i;
+        while (i > 0 && share(i) > end_unit) --i;
         hdr[blockIdx.x] = make_int4(seq, hk, rt, (int)(i - blockIdx.x + 1));
       }
       fence_proxy_async_smem();  // the merge buffer becomes the ring again: ordinary accesses before TMA writes

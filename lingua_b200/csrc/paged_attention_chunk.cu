@@ -41,11 +41,6 @@ struct CkCfg {
   static constexpr int SLOT = 256 * D + 512;  // floats of a partial result: O, row maxima, row sums
 };
 
-// a / b of non-negative numbers; 64-bit division is a long subroutine
-__device__ __forceinline__ long long ck_div(long long a, long long b) {
-  return (unsigned long long)a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
-
 struct CkSeq {
   int q0, nq, pos0, end;  // first row of q, new tokens, position of the first one, end of the readable keys
 };
@@ -208,7 +203,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   }
   const long long n_blocks = max(1ll, min((long long)gridDim.x, total));  // no share is empty
   const bool busy = blockIdx.x < n_blocks;
-  auto share = [&](long long i) { return ck_div(total * i, n_blocks); };  // first unit of share i
+  auto share = [&](long long i) { return div_nonneg(total * i, n_blocks); };  // first unit of share i
   const long long u0 = busy ? share(blockIdx.x) : 0, u1 = busy ? share(blockIdx.x + 1) : 0;
   if (u0 < u1 && u0 >= before && u0 < before + mine) {
     long long at = before;
@@ -222,7 +217,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         const long long one = seq_tiles(q);
         if (u0 < at + a.Hkv * one) {
           found = true;
-          const int hk = (int)ck_div(u0 - at, one);
+          const int hk = (int)div_nonneg(u0 - at, one);
           long long rest = u0 - at - hk * one;  // units of this head before u0
           const int n_pairs = (q.nq + 2 * tpt - 1) / (2 * tpt);
           for (int p0 = 0; p0 < n_pairs; p0 += 32) {
@@ -633,7 +628,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       tc_fence_before();  // O has been read: the next piece's products, ordered after the next p_half, may overwrite it
       if (!whole && i0 == 0 && threadIdx.x == 128) {
         const long long end_unit = u1 - w.left - w.first + t.nt + CK_ITEM_COST - 1;  // last unit of this item
-        long long i = ck_div(end_unit * n_blocks, total);           // share it belongs to
+        long long i = div_nonneg(end_unit * n_blocks, total);           // share it belongs to
         while (i + 1 < n_blocks && share(i + 1) <= end_unit) ++i;
         while (i > 0 && share(i) > end_unit) --i;
         hdr[blockIdx.x] = make_int4(w.seq, w.hk, w.pair, (int)(i - blockIdx.x + 1));
