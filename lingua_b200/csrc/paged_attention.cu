@@ -14,7 +14,8 @@
 //    item that crosses a share boundary leaves partial results (running maximum, sum, unnormalised output, fp32) that
 //    a second small kernel joins. The shares follow from the lengths on the device: a captured graph can be replayed with
 //    other lengths. When the table's width allows no item longer than NOSPLIT_BLOCKS blocks, items are dealt out whole
-//    instead and the second kernel is not launched.
+//    instead and the second kernel is not launched. A few sequences of moderate length (one token each) are cut by
+//    clusters: up to 8 blocks share an item and join their parts through distributed shared memory, in one launch.
 //  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. Every warp
 //    keeps its own ring of 16-key stages in shared memory, filled by TMA (boxes of 16 keys x 64 channels, 128-byte
 //    swizzle), so a stage is waited for and given back by one warp alone.
@@ -64,6 +65,26 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_cluster(uint32_t saddr, int rank) {  // the same address in block `rank`'s shared memory
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a)
+               : "memory");
+  return v;
+}
+
 // What a sequence asks for.
 struct DecSeq {
   int q0, nq;       // its rows of q
@@ -100,9 +121,8 @@ __device__ __forceinline__ DecSeq dec_seq(const LbPagedAttnArgs& a, int s, bool 
 }
 
 struct DecWork {  // found by one thread, read by the block
-  long long first, last;  // this block's share of the units [first, last)
-  int seq;                // sequence of `first`
-  long long offset;       // units of that sequence before `first`
+  int seq;           // sequence of this block's first unit
+  long long offset;  // units of that sequence before it
 };
 
 // Workspace: per block two partial results (its first item when an earlier block began it, its last item when a later
@@ -110,7 +130,7 @@ struct DecWork {  // found by one thread, read by the block
 template <int D, int NT>
 __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_constant__ CUtensorMap tk,
                                                               const __grid_constant__ CUtensorMap tv,
-                                                              const LbPagedAttnArgs a, float* ws, int4* hdr) {
+                                                              const LbPagedAttnArgs a, float* ws, int4* hdr, int cl) {
   using Cfg = DecCfg<D, NT>;
   constexpr int ROWS = Cfg::ROWS;
   extern __shared__ uint8_t dyn[];
@@ -119,10 +139,11 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   __shared__ long long warp_sum[4];
   __shared__ DecWork work;
   __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+  __shared__ float part_m[ROWS], part_l[ROWS];  // of this block's part of a cluster's item
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int G = a.H / a.Hkv;
-  const bool split = ws != nullptr;
+  const bool split = ws != nullptr || cl;  // cl: blocks of a cluster that share an item, 0 without clusters
   const uint32_t dyn0 = (smem_u32(dyn) + 1023u) & ~1023u;  // the swizzle pattern repeats every 1024 bytes
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -135,6 +156,17 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this block's share: a unit is one 64-key block of an item (or a whole item without splitting)
+  long long u0, u1, total = 0, n_blocks = 1;
+  auto share = [&](long long i) { return div_nonneg(total * i, n_blocks); };  // first unit of share i
+  if (cl) {
+    const int item = blockIdx.x / cl, rank = blockIdx.x % cl, per_seq = gridDim.x / (a.n_seqs * cl);
+    const int s = item / per_seq;
+    const DecSeq q = dec_seq<ROWS>(a, s, rank == 0 && item % per_seq == 0);
+    u0 = (long long)q.nb * rank / cl;
+    u1 = (long long)q.nb * (rank + 1) / cl;
+    if (threadIdx.x == 0) { work.seq = s; work.offset = (long long)(item % per_seq) * q.nb + u0; }
+    if (threadIdx.x < ROWS) { part_m[threadIdx.x] = -INFINITY; part_l[threadIdx.x] = 0.f; }
+  } else {
   const int per = (a.n_seqs + 127) / 128;
   const int s_lo = min(a.n_seqs, (int)threadIdx.x * per), s_hi = min(a.n_seqs, s_lo + per);
   long long mine = 0;
@@ -150,7 +182,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   }
   if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  long long before = 0, total = 0;
+  long long before = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     if (w < warp) before += warp_sum[w];
@@ -158,18 +190,19 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   }
   before += incl - mine;
   // no share is empty (the join kernel counts on that)
-  const long long n_blocks = max(1ll, min((long long)gridDim.x, total));
+  n_blocks = max(1ll, min((long long)gridDim.x, total));
   const bool busy = blockIdx.x < n_blocks;
-  auto share = [&](long long i) { return div_nonneg(total * i, n_blocks); };  // first unit of share i
-  const long long u0 = busy ? share(blockIdx.x) : 0, u1 = busy ? share(blockIdx.x + 1) : 0;
+  u0 = busy ? share(blockIdx.x) : 0;
+  u1 = busy ? share(blockIdx.x + 1) : 0;
   if (u0 < u1 && u0 >= before && u0 < before + mine) {
     long long at = before;
     for (int s = s_lo; s < s_hi; ++s) {
       const DecSeq q = dec_seq<ROWS>(a, s, false);
       const long long n = (long long)a.Hkv * q.rt * (split ? q.nb : 1);
-      if (u0 < at + n) { work.first = u0; work.last = u1; work.seq = s; work.offset = u0 - at; break; }
+      if (u0 < at + n) { work.seq = s; work.offset = u0 - at; break; }
       at += n;
     }
+  }
   }
   // rows of q that belong to no sequence
   if (a.cu_q) {
@@ -181,10 +214,11 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
       for (long long i = threadIdx.x; i < vec; i += 128) row[i] = make_uint4(0, 0, 0, 0);
     }
   }
-  if (split && threadIdx.x == 0) hdr[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (hdr && threadIdx.x == 0) hdr[blockIdx.x] = make_int4(0, 0, 0, 0);
   __syncthreads();
-  if (u0 >= u1) return;
+  if (u0 >= u1 && !cl) return;
 
+  float* obuf = reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)));  // the ring, once an item's blocks are done
   const uint32_t ring = dyn0 + warp * (Cfg::NST * Cfg::STAGE);
   const uint32_t bars = smem_u32(&full[warp][0]);
   uint32_t parity = 0;  // bit st: phase the next wait on stage st completes
@@ -393,8 +427,11 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
           if (r == 0) { sm_m[warp][8 * t + 2 * c + i] = m[t][i]; sm_l[warp][8 * t + 2 * c + i] = l[t][i]; }
         }
       __syncthreads();
-      if (abort_flag) return;  // read by all after the same barrier
-      float* obuf = reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)));
+      if (abort_flag) {  // read by all after the same barrier
+        if (!cl) return;
+        left = 0;  // the other blocks of the cluster are met below; this one has nothing to add
+        break;
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -413,7 +450,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         }
       __syncthreads();
       const bool whole_item = b0 == 0 && b1 == q.nb;
-      float* slot = whole_item ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
+      float* slot = whole_item || cl ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
       for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
         const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
         const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
@@ -425,7 +462,10 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
           o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
           L += sm_m[w][row] == -INFINITY ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);
         }
-        if (whole_item) {
+        if (cl) {  // nobody else reads or writes these four floats of the merge buffer
+          *reinterpret_cast<float4*>(obuf + row * Cfg::OROW + ch) = o;
+          if (ch == 0) { part_m[row] = M; part_l[row] = L; }
+        } else if (whole_item) {
           const float inv = L > 0.f ? 1.f / L : 0.f;
           const int gr = row0 + row;
           __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
@@ -435,6 +475,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
           if (ch == 0) { slot[ROWS * D + row] = M; slot[ROWS * D + ROWS + row] = L; }
         }
       }
+      if (cl) break;
       if (!whole_item && b0 == 0 && threadIdx.x == 0) {
         // units [u1 - (b1 - b0), + nb) hold this item: find the block its last unit belongs to
         const long long end_unit = u1 - (b1 - b0) + q.nb - 1;
@@ -448,6 +489,47 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
       __syncthreads();
     }
   }
+  if (!cl) return;
+
+  // ---- join the cluster's parts: every block is met here, whatever became of its part, and each writes a slice
+  cluster_sync();
+  {
+    const int item = blockIdx.x / cl, rank = blockIdx.x % cl, per_seq = gridDim.x / (a.n_seqs * cl);
+    const DecSeq q = dec_seq<ROWS>(a, item / per_seq, false);
+    const int hk = (item % per_seq) / q.rt, row0 = (item % per_seq) % q.rt * ROWS;
+    const int n_rows = min(ROWS, q.nq * G - row0);
+    const uint32_t pm = smem_u32(part_m), pl = smem_u32(part_l), po = smem_u32(obuf);
+    for (int i = threadIdx.x + 128 * rank; i < n_rows * (D / 4); i += 128 * cl) {
+      const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
+      // all parts' loads in flight at once; the buffer of a part that saw no key may hold anything
+      float m[8], l[8], M = -INFINITY, L = 0.f;
+      float4 x[8], o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        m[p] = -INFINITY;
+        if (p < cl) {
+          m[p] = ld_cluster(map_cluster(pm + 4 * row, p));
+          l[p] = ld_cluster(map_cluster(pl + 4 * row, p));
+          x[p] = ld_cluster4(map_cluster(po + 4 * (row * Cfg::OROW + ch), p));
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 8; ++p) M = fmaxf(M, m[p]);
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        if (m[p] != -INFINITY) {
+          const float f = exp2f(m[p] - M);
+          L += f * l[p];
+          o.x += f * x[p].x; o.y += f * x[p].y; o.z += f * x[p].z; o.w += f * x[p].w;
+        }
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const int gr = row0 + row;
+      __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
+      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
+  }
+  cluster_sync();  // nobody leaves while its shared memory is being read
 }
 
 // Joins the parts of the item that block `blockIdx.x` of the kernel above began and later blocks went on with: warps
@@ -502,7 +584,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAtt
 }
 
 template <int D, int NT>
-static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
+static int launch_decode(const LbPagedAttnArgs& a, void* ws, int cl, cudaStream_t st) {
   using Cfg = DecCfg<D, NT>;
   if (ensure_dyn_smem<paged_decode_kernel<D, NT>>(Cfg::SMEM)) return 20;
   const int grid = 2 * num_sms();
@@ -511,7 +593,23 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, cudaStream_t st) {
   CUtensorMap tk, tv;
   if (make_tmap_4d(&tk, a.k_pages, 2, D, a.page, a.kp_st, a.Hkv, a.kp_sh, a.n_pages, a.kp_sp, 64, 16)) return 10;
   if (make_tmap_4d(&tv, a.v_pages, 2, D, a.page, a.vp_st, a.Hkv, a.vp_sh, a.n_pages, a.vp_sp, 64, 16)) return 11;
-  paged_decode_kernel<D, NT><<<grid, 128, Cfg::SMEM, st>>>(tk, tv, a, (float*)ws, hdr);
+  if (cl) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_seqs * a.Hkv * ((a.H / a.Hkv + Cfg::ROWS - 1) / Cfg::ROWS) * cl);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cl;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, NT>, tk, tv, a, (float*)nullptr, (int4*)nullptr, cl);
+    if (e != cudaSuccess) return 400 + (int)e;
+  } else {
+    paged_decode_kernel<D, NT><<<grid, 128, Cfg::SMEM, st>>>(tk, tv, a, (float*)ws, hdr, 0);
+  }
   g_launches.fetch_add(1, std::memory_order_relaxed);
   if (ws) {
     // starts while the first kernel's last blocks run, and waits for all of it before it reads
@@ -553,6 +651,24 @@ static bool use_chunk(const LbPagedAttnArgs& a) {
 }
 // one row tile of 8 where that holds all rows of a sequence, else of 16
 static bool eight_rows(const LbPagedAttnArgs& a) { return (long long)(a.cu_q ? a.max_q : 1) * (a.H / a.Hkv) <= 8; }
+// most 64-key blocks an item can have
+static long long most_blocks(const LbPagedAttnArgs& a) {
+  long long keys = (long long)a.cols * a.page;
+  if (a.window > 0 && !a.cu_q) keys = std::min(keys, (long long)a.window + a.sinks + DEC_BLOCK);
+  return (keys + DEC_BLOCK - 1) / DEC_BLOCK;
+}
+// Blocks of a cluster that share an item; 0: no clusters. For one token per sequence, and as long as a block of the
+// cluster has no more than FEW_BLOCKS key blocks and the clusters fit the GPU side by side; beyond that equal shares of
+// everything are worth the second launch.
+static int cluster_size(const LbPagedAttnArgs& a) {
+  const long long blocks = most_blocks(a);
+  if (a.cu_q || blocks <= NOSPLIT_BLOCKS) return 0;
+  const int rows = eight_rows(a) ? 8 : 16;
+  const long long items = (long long)a.n_seqs * a.Hkv * ((a.H / a.Hkv + rows - 1) / rows);
+  for (int cl = 8; cl > 1; cl /= 2)
+    if (items * cl <= 2ll * num_sms() && blocks <= (long long)cl * FEW_BLOCKS) return cl;
+  return 0;
+}
 template <int NT>
 static long long decode_slot(int D) { return D == 128 ? DecCfg<128, NT>::SLOT : DecCfg<64, NT>::SLOT; }
 }  // namespace lb
@@ -560,9 +676,7 @@ static long long decode_slot(int D) { return D == 128 ? DecCfg<128, NT>::SLOT : 
 extern "C" long long lb_paged_attention_workspace(const LbPagedAttnArgs* a) {
   using namespace lb;
   if (use_chunk(*a)) return paged_chunk_workspace(a->D);
-  long long keys = (long long)a->cols * a->page;  // most keys a row can see
-  if (a->window > 0 && !a->cu_q) keys = std::min(keys, (long long)a->window + a->sinks);
-  if (keys <= NOSPLIT_BLOCKS * DEC_BLOCK) return 0;
+  if (most_blocks(*a) <= NOSPLIT_BLOCKS || cluster_size(*a)) return 0;
   const long long slot = eight_rows(*a) ? decode_slot<1>(a->D) : decode_slot<2>(a->D);
   return 2ll * num_sms() * (2 * slot * 4 + 16);
 }
@@ -576,7 +690,8 @@ extern "C" int lb_paged_attention(const LbPagedAttnArgs* a, void* workspace, voi
   if (a->T <= 0) return 0;
   if (use_chunk(*a)) return workspace ? paged_chunk_dispatch(*a, workspace, (cudaStream_t)stream) : 5;
   cudaStream_t st = (cudaStream_t)stream;
+  const int cl = cluster_size(*a);
   if (eight_rows(*a))
-    return a->D == 128 ? launch_decode<128, 1>(*a, workspace, st) : launch_decode<64, 1>(*a, workspace, st);
-  return a->D == 128 ? launch_decode<128, 2>(*a, workspace, st) : launch_decode<64, 2>(*a, workspace, st);
+    return a->D == 128 ? launch_decode<128, 1>(*a, workspace, cl, st) : launch_decode<64, 1>(*a, workspace, cl, st);
+  return a->D == 128 ? launch_decode<128, 2>(*a, workspace, cl, st) : launch_decode<64, 2>(*a, workspace, cl, st);
 }
