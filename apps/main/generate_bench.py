@@ -1,7 +1,7 @@
 """Generation throughput of the packed KV-cache generator on a random-init model.
 
     python -m apps.main.generate_bench [--model 1b|7b|hawk_1b|mingru_1b|minlstm_1b|mamba_1b] [--batch 32]
-                                       [--prompt 512] [--new 256]
+                                       [--prompt 512] [--new 256] [--page-size 64]
 
 Times ``PackedCausalTransformerGenerator.generate`` (prefill of all prompts packed in one sequence, then one
 decode step per new token for the whole batch; apps/main/generate.py:310-420 of the reference) with CUDA events
@@ -14,7 +14,7 @@ import json
 
 import torch
 
-from lingua_b200.generation import PackedCausalTransformerGenerator, PackedCausalTransformerGeneratorArgs
+from lingua_b200.generation import PackedCausalTransformerGeneratorArgs, build_generator
 from lingua_b200.models.transformer import LMTransformer, LMTransformerArgs
 from lingua_b200.tokenizer import build_tokenizer
 
@@ -47,9 +47,10 @@ def main(argv=None):
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--new", type=int, default=256)
     ap.add_argument("--eager", action="store_true", help="do not replay the decode step as a CUDA graph")
+    ap.add_argument("--page-size", type=int, default=0, help="paged KV cache with pages of this many tokens")
     a = ap.parse_args(argv)
     dev = torch.device("cuda")
-    gen_cls = PackedCausalTransformerGenerator
+    gen_cls = build_generator
     torch.manual_seed(0)
     if a.model in RECURRENT:
         import importlib
@@ -70,7 +71,7 @@ def main(argv=None):
     model.eval()
     tok = build_tokenizer("bytes")
     cfg = PackedCausalTransformerGeneratorArgs(temperature=0.0, max_gen_len=a.new, max_prompt_len=a.prompt,
-                                               max_tokens=a.batch * (a.prompt + a.new),
+                                               max_tokens=a.batch * (a.prompt + a.new + a.page_size), page_size=a.page_size,
                                                reduce_generation_overhead=not a.eager)
     gen = gen_cls(cfg, model, tok)
     g = torch.Generator().manual_seed(1)
@@ -90,7 +91,7 @@ def main(argv=None):
     n_new = a.batch * a.new
     # prefill alone, to separate the decode phase
     cfg0 = PackedCausalTransformerGeneratorArgs(temperature=0.0, max_gen_len=1, max_prompt_len=a.prompt,
-                                                max_tokens=a.batch * (a.prompt + 1))
+                                                max_tokens=a.batch * (a.prompt + 1 + a.page_size), page_size=a.page_size)
     gen0 = gen_cls(cfg0, model, tok)
     gen.release_cache()
     gen0.generate(prompts)
@@ -107,7 +108,7 @@ def main(argv=None):
         "prompt_tokens": a.prompt, "new_tokens": a.new, "ms_total": round(ms, 1), "ms_prefill": round(ms_prefill, 1),
         "tokens_per_s_end_to_end": round(n_new / ms * 1e3, 1),
         "tokens_per_s_decode": round(n_new / max(ms - ms_prefill, 1e-3) * 1e3, 1),
-        "ms_per_decode_step": round((ms - ms_prefill) / a.new, 3), "cuda_graph": not a.eager, "dtype": "bf16",
+        "ms_per_decode_step": round((ms - ms_prefill) / a.new, 3), "cuda_graph": not a.eager, "page_size": a.page_size, "dtype": "bf16",
         "data": "random prompts, random-init weights"}))
 
 

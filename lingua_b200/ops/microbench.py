@@ -5,7 +5,7 @@ than L2 or an L2 flush between iterations) and prints achieved TFLOP/s or GB/s n
 measured peaks of ``MEASURED_PEAKS.json`` when that file is present. It is also the small,
 self-terminating workload to put under ``ncu`` when profiling a single kernel.
 
-ops: gemm, gemm_wgrad, gemm_gather, gemm_scatter, gemm_tp_ag, gemm_tp_rs, rglru_gates, ssm_update, ssd, attn_fwd, attn_bwd, rmsnorm, rmsnorm_bwd, glu, ce, adamw, rope, scan, conv1d, decode
+ops: gemm, gemm_wgrad, gemm_gather, gemm_scatter, gemm_tp_ag, gemm_tp_rs, rglru_gates, ssm_update, ssd, attn_fwd, attn_bwd, rmsnorm, rmsnorm_bwd, glu, ce, adamw, rope, scan, conv1d, decode, paged_decode, paged_chunk, copy_pages, penalize
 """
 from __future__ import annotations
 
@@ -319,6 +319,39 @@ def main(argv=None):
                                                    start.data_ptr(), ln.data_ptr(), out.data_ptr(), nseq, H, H, 128,
                                                    H * 128, H * 128, 1 / math.sqrt(128), _lib.stream_ptr()), "decode")
         bytes_ = 2.0 * nseq * L * H * 128 * 2
+    elif a.op in ("paged_decode", "paged_chunk"):
+        # --batch sequences of --seq keys, --heads query heads on a quarter as many key heads; chunk: --m new tokens each
+        from .paged import paged_attention
+
+        n, H, Hkv, P, T = a.batch, a.heads, max(1, a.heads // 4), 64, 1 if a.op == "paged_decode" else min(a.m, a.seq)
+        pages = (a.seq + P - 1) // P
+        kp, vp = (torch.randn(n * pages, P, Hkv, 128, device=dev, dtype=bf) for _ in range(2))
+        table = torch.randperm(n * pages, device=dev).int().view(n, pages)
+        q = torch.randn(n * T, H, 128, device=dev, dtype=bf)
+        ln = torch.full((n,), a.seq, device=dev, dtype=torch.int32)
+        cu = None if T == 1 else (torch.arange(n + 1, device=dev) * T).int()
+        fn = lambda: paged_attention(q, kp, vp, table, ln, cu, T)
+        if T == 1:
+            bytes_ = 2.0 * n * a.seq * Hkv * 128 * 2
+        else:
+            flops = 4.0 * n * H * 128 * (T * a.seq - T * (T - 1) / 2)
+    elif a.op == "copy_pages":
+        from .paged import copy_pages
+
+        pool = torch.zeros(64, 128, 64, 8, 128, device=dev, dtype=bf)
+        ids = torch.randperm(128, device=dev).int()
+        fn = lambda: copy_pages(pool, ids[:64], ids[64:])
+        bytes_ = 2.0 * 64 * 64 * pool[0, 0].numel() * 2
+    elif a.op == "penalize":
+        from .logits import penalize_logits
+
+        rows, V, L = 64, 128256, 2000
+        x = torch.randn(rows, V, device=dev)
+        hist = torch.randint(0, V, (rows, L), device=dev)
+        ln = torch.full((rows,), L, device=dev, dtype=torch.int32)
+        ok = torch.randint(-2 ** 31, 2 ** 31, (rows, V // 32), device=dev).int()
+        fn = lambda: penalize_logits(x, hist, ln, repetition=1.2, presence=0.1, frequency=0.1, allowed=ok)
+        bytes_ = rows * V * (8 + 1 / 8) + 8.0 * rows * L
     else:
         raise SystemExit(f"unknown op {a.op}")
     ms = _time(fn, a.iters, flush)
