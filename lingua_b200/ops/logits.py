@@ -82,6 +82,7 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
         _refuse(t is not None and t.device != dev, "all tensors must be on one device")
     if out is not None:
         _refuse(out.shape != logits.shape or out.dtype != logits.dtype, "out must have the logits' shape and dtype")
+        _refuse(N > 1 and out.stride(0) < V, "rows of out must not overlap")
     _refuse(logits.requires_grad and torch.is_grad_enabled(), "penalize_logits has no gradient")
     if not logits.is_cuda:
         z = penalize_logits_ref(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, allowed)

@@ -26,6 +26,7 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
+MAX_POSITIONS = 1 << 30
 
 
 def _refuse(cond: bool, msg: str) -> None:
@@ -40,6 +41,10 @@ def _strided(t: torch.Tensor, name: str) -> None:
     for n, s in zip(t.shape[:-1], st[:-1]):
         ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
     _refuse(not ok, f"{name} needs contiguous channels, 16-byte aligned rows and positive strides, got {tuple(st)}")
+
+
+def _tracked(*ts: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -64,8 +69,8 @@ def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
                 and kv_len.get_device() == dev and kv_len.is_contiguous()
                 and (q.shape[0] == n if cu_q is None else cu_q.dtype is i32 and cu_q.shape == (n + 1,)
                      and cu_q.get_device() == dev and cu_q.is_contiguous())
-                and (block_table.stride(1) == 1 or block_table.shape[1] <= 1) and _aligned(q) and _aligned(k_pages)
-                and _aligned(v_pages) and not (q.requires_grad and torch.is_grad_enabled())):
+                and (block_table.stride(1) == 1 or block_table.shape[1] <= 1) and block_table.shape[1] * P <= MAX_POSITIONS
+                and _aligned(q) and _aligned(k_pages) and _aligned(v_pages) and not _tracked(q, k_pages, v_pages)):
             return
     _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
 
@@ -88,7 +93,8 @@ def _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
         _refuse(t is not None and t.device != dev, "all tensors must be on one device")
     dt = q.dtype
     _refuse(k_pages.dtype != dt or v_pages.dtype != dt, "tokens and cache must have one dtype")
-    _refuse(q.requires_grad and torch.is_grad_enabled(), "paged-cache operators have no gradient")
+    _refuse(_tracked(q, k_pages, v_pages), "paged-cache operators have no gradient")
+    _refuse(block_table.shape[1] * k_pages.shape[1] > MAX_POSITIONS, f"a sequence has at most {MAX_POSITIONS} positions")
     if not q.is_cuda:
         return
     _refuse(dt != torch.bfloat16, "the kernels take bf16")
@@ -171,7 +177,9 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     _refuse(k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D), "k and v must be [T, Hkv, D]")
     _refuse(k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device,
             "q, k and v must share dtype and device")
+    _refuse(_tracked(k, v), "paged-cache operators have no gradient")
     if cs is not None:
+        _refuse(cs.data_ptr() % 16 != 0 and cs.is_cuda, "cs must be 16-byte aligned")
         _refuse(cs.dtype != torch.float32 or cs.dim() != 3 or cs.shape[1:] != (D // 2, 2) or not cs.is_contiguous()
                 or cs.device != q.device, "cs must be a contiguous fp32 [positions, D / 2, 2] table")
     if not q.is_cuda:
@@ -236,6 +244,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     the kernel (a wrong value costs speed, not correctness)."""
     _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
     _refuse(window < 0 or sinks < 0, "window and sinks must not be negative")
+    window, sinks = window if window < MAX_POSITIONS else 0, min(sinks, MAX_POSITIONS)  # no position is further away
     T, H, D = q.shape
     n_pages, P, Hkv, _ = k_pages.shape
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
@@ -249,7 +258,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     args = _lib.PAGED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
         0 if cu_q is None else cu_q.data_ptr(), _status(dev),
-        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, max_q, scale,
+        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, min(max_q, MAX_POSITIONS), scale,
         block_table.stride(0), *q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
     lib = _lib.load()
     with _on(dev):
@@ -271,7 +280,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
     _refuse(pool.dim() < 2, "pool must be [rows, n_pages, ...]")
     _refuse(src.dim() != 1 or src.shape != dst.shape, "src and dst must be two lists of the same length")
     _refuse(src.dtype != torch.int32 or dst.dtype != torch.int32, "page ids must be int32")
-    _refuse(pool.requires_grad and torch.is_grad_enabled(), "copy_pages has no gradient")
+    _refuse(_tracked(pool), "copy_pages has no gradient")
     _refuse(src.device != dst.device, "src and dst must be on one device")
     rows, n_pages = pool.shape[:2]
     n = src.numel()

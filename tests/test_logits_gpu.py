@@ -87,4 +87,6 @@ def test_refusals_on_the_gpu():
                   ((X, Hh, Hl), dict(repetition=torch.ones(2))), ((X, Hh[:, ::2], Hl), {})):
         with pytest.raises(ValueError):
             penalize_logits(*a, **kw)
+    with pytest.raises(ValueError):
+        penalize_logits(X, Hh, Hl, out=torch.empty(1, 64, device=DEV).expand(2, 64))
     assert penalize_logits(X[:0], Hh[:0], Hl[:0]).shape == (0, 64)

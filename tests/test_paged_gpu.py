@@ -233,3 +233,83 @@ def test_refusals_on_the_gpu():
             P.copy_pages(pool, torch.tensor([0], dtype=torch.int32), torch.tensor([1], dtype=torch.int32))
     empty = make_batch([], [], 4, 2, 128, 16, DEV, poison=False)
     assert attend(empty, one=True).shape == (0, 4, 128)
+
+
+def test_further_refusals_on_the_gpu():
+    b = make_batch([1, 1], [20, 30], 4, 2, 128, 16, DEV, poison=False)
+    app = lambda **kw: P.paged_append(**{**dict(q=b["q"], k=b["k"], v=b["v"], k_pages=b["k_pages"], v_pages=b["v_pages"],
+                                                block_table=b["table"], kv_len=b["kv_len"], cs=rotary(64, 128, DEV)), **kw})
+    odd = torch.zeros(64 * 128 + 1, device=DEV)[1:].view(64, 64, 2)  # a rotary table that 16-byte loads cannot read
+    for kw in (dict(cs=odd), dict(k=b["k"].clone().requires_grad_(True)), dict(cs=rotary(64, 128)),
+               dict(k=torch.zeros(2 * 2 * 128 + 1, device=DEV).bfloat16()[1:].view(2, 2, 128)), dict(v=b["v"].float())):
+        with pytest.raises(ValueError):
+            app(**kw)
+    for kw in (dict(k_pages=b["k_pages"].clone().requires_grad_(True)),
+               dict(table=torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(2, 2 ** 27))):
+        with pytest.raises(ValueError):
+            attend({**b, **kw}, one=True)
+    for scale in (-0.1, float("nan")):
+        with pytest.raises(ValueError):
+            attend(b, one=True, scale=scale)
+    assert app().shape == (2, 4, 128)
+
+
+@pytest.mark.parametrize("q,kv", [([1, 1, 1], [300, 40, 7]), ([40, 1, 200], [300, 40, 200])])
+def test_no_sequences_rows_before_the_first_and_wide_limits(q, kv):
+    b = make_batch(q, kv, 8, 2, 128, 16, DEV, pad_rows=2, seed=5)
+    ref, mag = attention64(b)
+    # the largest window and as many first tokens as there can be change nothing
+    for kw in (dict(window=2 ** 31 - 1), dict(window=2 ** 40, sinks=2 ** 40), dict(window=5, sinks=2 ** 31 - 1)):
+        o = attend(b, **kw)
+        assert ((o.double() - ref).abs() <= attention_tolerance(ref, mag)).all()
+    # three rows in front that belong to nobody
+    front = {**b, "q": torch.cat((b["q"][:3], b["q"])), "cu_q": b["cu_q"] + 3}
+    o = attend(front)
+    assert (o[:3] == 0).all() and ((o[3:].double() - ref).abs() <= attention_tolerance(ref, mag)).all()
+    none = {**b, "table": b["table"][:0], "kv_len": b["kv_len"][:0], "cu_q": torch.zeros(1, dtype=torch.int32, device=DEV)}
+    assert (attend(none) == 0).all()
+    assert (P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], none["table"], none["kv_len"], none["cu_q"]) == 0).all()
+
+
+@pytest.mark.parametrize("G", [72, 128, 160])
+def test_large_groups(G):
+    b = make_batch([1, 3, 9], [50, 131, 9], G, 1, 128, 32, DEV, seed=G)
+    check(attend(b), b)
+
+
+@pytest.mark.parametrize("max_q", [0, 1, 2, 10 ** 6, 2 ** 40])
+def test_a_wrong_max_q_only_costs_time(max_q):
+    b = make_batch([1, 50, 3], [700, 600, 5], 8, 2, 128, 16, DEV, seed=8)
+    o = P.paged_attention(b["q"], b["k_pages"], b["v_pages"], b["table"], b["kv_len"], cu_q=b["cu_q"], max_q=max_q)
+    check(o, b)
+
+
+def test_one_token_batches_of_every_split():
+    """Whole items, clusters of 2 to 8 and equal shares, with lengths far below what the table allows."""
+    for n, cols in ((1, 300), (3, 40), (9, 40), (18, 40), (40, 40), (150, 40), (7, 3)):
+        kv = [(i * 61 + 1) % min(16 * cols, 700) for i in range(n)]
+        b = make_batch([1] * n, kv, 16, 8, 128, 16, DEV, seed=n)
+        wide = torch.full((n, cols), -5, dtype=torch.int32, device=DEV)
+        w = min(cols, b["table"].shape[1])
+        wide[:, :w] = b["table"][:, :w]
+        check(attend({**b, "table": wide}, one=True), b)
+
+
+def test_offsets_past_32_bits():
+    """The last pages of a pool of more than 2^31 elements, through every operator."""
+    page, Hkv, D, n_pages = 64, 8, 128, 2 ** 31 // (64 * 8 * 128) + 40
+    pool = torch.empty(2, n_pages, page, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    last = torch.arange(n_pages - 20, n_pages, device=DEV).int()
+    for q, kv in (([1, 1], [300, 129]), ([70, 200], [300, 700])):
+        b = make_batch(q, kv, 16, Hkv, D, page, DEV, poison=False)
+        old, used = b["table"], b["k_pages"].shape[0]
+        assert used <= 20
+        pool[0, last[:used].long()], pool[1, last[:used].long()] = b["k_pages"], b["v_pages"]
+        big = {**b, "k_pages": pool[0], "v_pages": pool[1], "table": torch.where(old >= 0, last[old.long().clamp(min=0)], old)}
+        P.paged_append(b["q"], b["k"], b["v"], b["k_pages"], b["v_pages"], old, b["kv_len"], b["cu_q"])
+        P.paged_append(b["q"], b["k"], b["v"], pool[0], pool[1], big["table"], b["kv_len"], b["cu_q"])
+        assert torch.equal(pool[0, last[:used].long()], b["k_pages"]) and torch.equal(pool[1, last[:used].long()], b["v_pages"])
+        assert torch.equal(attend(big), attend(b))
+    P.copy_pages(pool, last[:3].contiguous(), torch.tensor([0, 5, n_pages - 1], dtype=torch.int32, device=DEV))
+    for s, d in zip(last[:3].tolist(), (0, 5, n_pages - 1)):
+        assert torch.equal(pool[:, d], pool[:, s])
