@@ -25,9 +25,9 @@ namespace lb {
 
 // Control warpgroup (a TMA warp, an MMA warp, two idle ones) and two softmax warpgroups. A softmax thread holds 128
 // scores: registers move from the control warps to it, within what the block was launched with (384 x 168 =
-// 128 x 88 + 256 x 208).
+// 128 x 104 + 256 x 200).
 constexpr int CK_THREADS = 384;
-constexpr int CK_REGS_CONTROL = 88, CK_REGS_SOFTMAX = 208;
+constexpr int CK_REGS_CONTROL = 104, CK_REGS_SOFTMAX = 200;
 constexpr int CK_ITEM_COST = 3;     // what beginning and ending an item costs, in key tiles (about 5 us against 1.9 us)
 constexpr int CK_HALF = 128 * 128;  // 128 rows x 64 channels: one swizzled box of a tile
 constexpr float CK_LOG2E = 1.4426950408889634f;
@@ -347,13 +347,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA
       if (elect_one()) {
-        uint32_t kv = 0, piece = 0, n_p[2] = {0, 0};
+        uint32_t kv = 0, piece = 0, n_p0 = 0, n_p1 = 0;
         walk([&](const CkSeq& q, const CkItem& t, const CkWalk& w, int i0, int i1) {
-          int last[2] = {-1, -1};  // last active key tile of each query tile
-          for (int s = 0; s < (t.n_tok1 > 0 ? 2 : 1); ++s)
-            for (int i = i1 - 1; i >= i0 && last[s] < 0; --i)
-              if (ck_active(a, t, s, ck_tile(t, i))) last[s] = i;
-          bool begun[2] = {false, false};
+          int last0 = -1, last1 = -1;  // last active key tile of each query tile
+          for (int i = i1 - 1; i >= i0 && last0 < 0; --i)
+            if (ck_active(a, t, 0, ck_tile(t, i))) last0 = i;
+          for (int i = i1 - 1; i >= i0 && last1 < 0 && t.n_tok1 > 0; --i)
+            if (ck_active(a, t, 1, ck_tile(t, i))) last1 = i;
+          bool begun0 = false, begun1 = false;
           // MMAs of one thread run in issue order: S_t(i + 1) overwrites P_t(i) only after O_t += P_t V(i) has read it, and
           // a commit after S_t(i + 1) also covers that product.
           auto issue_s = [&](int s, int st) {
@@ -362,20 +363,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             for (int k = 0; k < D / 16; ++k) umma_f16(tS(s), ck_slice_k(dq, k), ck_slice_k(dk, k), IDESC_S, k != 0);
             umma_commit(s_full(s));
           };
-          auto issue_pv = [&](int s, int st, int i) -> bool {
-              // the first 64 keys' P is multiplied while the softmax warps are still at the other 64
+          auto issue_pv = [&](int s, int st, uint32_t& n_p, bool& begun, bool last) -> bool {
+            // the first 64 keys' P is multiplied while the softmax warps are still at the other 64
             const uint64_t dv = make_smem_desc(sV(st), CK_HALF, 1024);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-              if (!mbar_wait(hf ? p_full(s) : p_half(s), n_p[s] & 1, &abort_flag, a.status, 0x64)) return false;
+              if (!mbar_wait(hf ? p_full(s) : p_half(s), n_p & 1, &abort_flag, a.status, 0x64)) return false;
               tc_fence_after();
 #pragma unroll
               for (int k = 4 * hf; k < 4 * hf + 4; ++k)
-                umma_f16_ts(tO(s), tS(s) + k * 8, ck_slice_mn(dv, k), IDESC_O, (begun[s] || k != 0) ? 1u : 0u);
+                umma_f16_ts(tO(s), tS(s) + k * 8, ck_slice_mn(dv, k), IDESC_O, (begun || k != 0) ? 1u : 0u);
             }
-            begun[s] = true;
-            ++n_p[s];
-            if (i == last[s]) umma_commit(o_done(s));
+            begun = true;
+            ++n_p;
+            if (last) umma_commit(o_done(s));
             return true;
           };
           auto scores = [&](int i, int s, bool& ready) -> bool {  // S of query tile s for key tile i
@@ -403,9 +404,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             ready = false;
             if (!mbar_wait(v_full(st), (n / NST) & 1, &abort_flag, a.status, 0x67)) return false;
             tc_fence_after();
-            if (a0 && !issue_pv(0, st, i)) return false;
+            if (a0 && !issue_pv(0, st, n_p0, begun0, i == last0)) return false;
             if (i + 1 < i1 && !scores(i + 1, 0, ready)) return false;
-            if (a1 && !issue_pv(1, st, i)) return false;
+            if (a1 && !issue_pv(1, st, n_p1, begun1, i == last1)) return false;
             umma_commit(v_empty(st));
             if (i + 1 < i1 && !scores(i + 1, 1, ready)) return false;
           }
