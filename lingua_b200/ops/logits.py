@@ -9,20 +9,26 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .paged import _on, _refuse
+from .paged import _on, _refuse, _tracked
 
 Knob = Optional[Union[float, torch.Tensor]]
 
 
-def _knob(value: Knob, name: str, N: int, neutral: float, dev):
+def _knob(value: Knob, name: str, N: int, neutral: float, dev: int):
     """(per-row tensor or None, scalar) of a penalty given as a number, an fp32 [N] tensor or None."""
     if value is None:
         return None, neutral
     if isinstance(value, torch.Tensor):
-        _refuse(value.shape != (N,) or value.dtype != torch.float32 or not value.is_contiguous() or value.device != dev,
-                f"{name} must be a number or a contiguous fp32 [N] tensor on the logits' device")
+        if value.shape != (N,) or value.dtype is not torch.float32 or not value.is_contiguous() or value.get_device() != dev:
+            raise ValueError(f"{name} must be a number or a contiguous fp32 [N] tensor on the logits' device")
         return value, neutral
     return None, float(value)
+
+
+def _rows(t: Optional[torch.Tensor], dtype: torch.dtype, shape, dev: int) -> bool:
+    """An operand that is absent, or as the kernel reads it: rows of ``shape`` without gaps inside them."""
+    return t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == dev
+                         and (shape[-1] <= 1 or t.stride(-1) == 1))
 
 
 def penalize_logits_ref(logits, history, history_len, prompt_len=None, repetition=None, presence=None, frequency=None,
@@ -66,42 +72,49 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
     The penalties are numbers or fp32 [N] tensors. A row whose mask allows nothing comes out as -inf everywhere."""
     _refuse(logits.dim() != 2, "logits must be [N, V]")
     N, V = logits.shape
-    dev = logits.device
-    _refuse(history.dim() != 2 or history.shape[0] != N or history.dtype != torch.int64, "history must be int64 [N, L]")
-    for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):
-        _refuse(t is not None and (t.shape != (N,) or t.dtype != torch.int32), f"{name} must be int32 [N]")
+    dev, dt = logits.get_device(), logits.dtype
     rep_t, rep = _knob(repetition, "repetition", N, 1.0, dev)
     _refuse(rep_t is None and not rep > 0.0, "repetition must be positive")
     pres_t, pres = _knob(presence, "presence", N, 0.0, dev)
     freq_t, freq = _knob(frequency, "frequency", N, 0.0, dev)
-    if bias is not None:
-        _refuse(bias.dtype != torch.float32 or bias.shape not in ((V,), (N, V)), "bias must be fp32 [V] or [N, V]")
-    if allowed is not None:
-        _refuse(allowed.dtype != torch.int32 or allowed.shape != (N, (V + 31) // 32), "allowed must be int32 [N, ceil(V / 32)]")
-    for t in (history, history_len, prompt_len, bias, allowed, out):
-        _refuse(t is not None and t.device != dev, "all tensors must be on one device")
-    if out is not None:
-        _refuse(out.shape != logits.shape or out.dtype != logits.dtype, "out must have the logits' shape and dtype")
-        _refuse(N > 1 and out.stride(0) < V, "rows of out must not overlap")
-    _refuse(logits.requires_grad and torch.is_grad_enabled(), "penalize_logits has no gradient")
-    if not logits.is_cuda:
-        z = penalize_logits_ref(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, allowed)
-        return z if out is None else out.copy_(z)
-    _refuse(logits.dtype not in (torch.bfloat16, torch.float32), "the kernel takes bf16 and fp32 logits")
-    _refuse(N > 65535, "too many rows")
-    for t in (logits, history, history_len, prompt_len, bias, allowed, out):
-        _refuse(t is not None and t.shape[-1] > 1 and t.stride(-1) != 1, "rows must be contiguous")
+    i32 = torch.int32
+    if not (dev >= 0 and (dt is torch.bfloat16 or dt is torch.float32) and N <= 65535 and history.dim() == 2
+            and _rows(logits, dt, (N, V), dev) and _rows(history, torch.int64, (N, history.shape[1]), dev)
+            and _rows(history_len, i32, (N,), dev) and _rows(prompt_len, i32, (N,), dev)
+            and (bias is None or _rows(bias, torch.float32, (V,) if bias.dim() == 1 else (N, V), dev))
+            and _rows(allowed, i32, (N, (V + 31) // 32), dev)
+            and _rows(out, dt, (N, V), dev) and (out is None or N <= 1 or out.stride(0) >= V) and not _tracked(logits)):
+        # something is unusual: the reference path, or words for what is wrong
+        _refuse(history.dim() != 2 or history.shape[0] != N or history.dtype != torch.int64, "history must be int64 [N, L]")
+        for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):
+            _refuse(t is not None and (t.shape != (N,) or t.dtype != i32), f"{name} must be int32 [N]")
+        _refuse(bias is not None and (bias.dtype != torch.float32 or bias.shape not in ((V,), (N, V))),
+                "bias must be fp32 [V] or [N, V]")
+        _refuse(allowed is not None and (allowed.dtype != i32 or allowed.shape != (N, (V + 31) // 32)),
+                "allowed must be int32 [N, ceil(V / 32)]")
+        for t in (history, history_len, prompt_len, bias, allowed, out):
+            _refuse(t is not None and t.device != logits.device, "all tensors must be on one device")
+        if out is not None:
+            _refuse(out.shape != logits.shape or out.dtype != dt, "out must have the logits' shape and dtype")
+            _refuse(N > 1 and out.stride(0) < V, "rows of out must not overlap")
+        _refuse(_tracked(logits), "penalize_logits has no gradient")
+        if not logits.is_cuda:
+            z = penalize_logits_ref(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, allowed)
+            return z if out is None else out.copy_(z)
+        _refuse(dt not in (torch.bfloat16, torch.float32), "the kernel takes bf16 and fp32 logits")
+        _refuse(N > 65535, "too many rows")
+        raise ValueError("rows must be contiguous")
     if out is None:
-        out = torch.empty((N, V), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((N, V))
     if N == 0 or V == 0:
         return out
     args = _lib.PENALIZE_ARGS.pack(
         logits.data_ptr(), out.data_ptr(), history.data_ptr(), history_len.data_ptr(),
-        *(0 if t is None else t.data_ptr() for t in (prompt_len, rep_t, pres_t, freq_t, bias, allowed)), N, V,
-        history.shape[1], _lib.LB_BF16 if logits.dtype == torch.bfloat16 else _lib.LB_F32, rep, pres, freq,
+        *[0 if t is None else t.data_ptr() for t in (prompt_len, rep_t, pres_t, freq_t, bias, allowed)], N, V,
+        history.shape[1], _lib.LB_BF16 if dt is torch.bfloat16 else _lib.LB_F32, rep, pres, freq,
         logits.stride(0), out.stride(0), history.stride(0), 0 if bias is None or bias.dim() == 1 else bias.stride(0),
         0 if allowed is None else allowed.stride(0))
-    with _on(logits.get_device()):
+    with _on(dev):
         rc = _lib.load().lb_penalize_logits(args, _lib.stream_ptr())
     _lib.check(rc, "lb_penalize_logits")
     return out

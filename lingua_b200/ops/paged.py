@@ -44,7 +44,11 @@ def _strided(t: torch.Tensor, name: str) -> None:
 
 
 def _tracked(*ts: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                return True
+    return False
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -174,23 +178,26 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
     T, H, D = q.shape
     n_pages, P, Hkv, _ = k_pages.shape
-    _refuse(k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D), "k and v must be [T, Hkv, D]")
-    _refuse(k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device,
-            "q, k and v must share dtype and device")
-    _refuse(_tracked(k, v), "paged-cache operators have no gradient")
-    if cs is not None:
-        _refuse(cs.data_ptr() % 16 != 0 and cs.is_cuda, "cs must be 16-byte aligned")
-        _refuse(cs.dtype != torch.float32 or cs.dim() != 3 or cs.shape[1:] != (D // 2, 2) or not cs.is_contiguous()
-                or cs.device != q.device, "cs must be a contiguous fp32 [positions, D / 2, 2] table")
-    if not q.is_cuda:
-        return paged_append_ref(q, k, v, k_pages, v_pages, block_table, kv_len, cu_q, cs)
-    if not (_aligned(k) and _aligned(v)):
+    dev, dt, shape = q.get_device(), q.dtype, (T, Hkv, D)
+    if not (dev >= 0 and k.shape == shape and v.shape == shape and k.dtype is dt and v.dtype is dt and k.get_device() == dev
+            and v.get_device() == dev and _aligned(k) and _aligned(v) and not _tracked(k, v)
+            and (cs is None or (cs.dtype is torch.float32 and cs.dim() == 3 and cs.shape[1] == D // 2 and cs.shape[2] == 2
+                                and cs.is_contiguous() and cs.get_device() == dev and cs.data_ptr() % 16 == 0))):
+        _refuse(k.shape != shape or v.shape != shape, "k and v must be [T, Hkv, D]")
+        _refuse(k.dtype != dt or v.dtype != dt or k.device != q.device or v.device != q.device,
+                "q, k and v must share dtype and device")
+        _refuse(_tracked(k, v), "paged-cache operators have no gradient")
+        if cs is not None:
+            _refuse(cs.dtype != torch.float32 or cs.dim() != 3 or cs.shape[1:] != (D // 2, 2) or not cs.is_contiguous()
+                    or cs.device != q.device, "cs must be a contiguous fp32 [positions, D / 2, 2] table")
+        if not q.is_cuda:
+            return paged_append_ref(q, k, v, k_pages, v_pages, block_table, kv_len, cu_q, cs)
+        _refuse(cs is not None and cs.data_ptr() % 16 != 0, "cs must be 16-byte aligned")
         _strided(k, "k")
         _strided(v, "v")
-    out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((T, H, D))
     if T == 0:
         return out
-    dev = q.get_device()
     args = _lib.PAGED_APPEND_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
         block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
@@ -251,7 +258,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _refuse(not scale >= 0.0, "scale must not be negative")
     if not q.is_cuda:
         return paged_attention_ref(q, k_pages, v_pages, block_table, kv_len, cu_q, scale, window, sinks)
-    out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((T, H, D))
     if T == 0:
         return out
     dev = q.get_device()
