@@ -31,7 +31,9 @@
 namespace lb {
 
 constexpr int DEC_BLOCK = 64;       // keys per block: 16 for each warp
-constexpr int NOSPLIT_BLOCKS = 4;  // 256 keys: 7.2 us whole, 7.9 us cut up; 511 keys 10.1 / 7.7 us (one sequence, 16 heads)
+// Items of up to so many blocks are not cut up: 256 keys 7.2 us whole, 7.9 us cut up; 511 keys 10.1 / 7.7 us, 6.5 us by clusters
+// (one sequence, 16 heads, in a graph).
+constexpr int NOSPLIT_BLOCKS = 4;
 constexpr float DEC_LOG2E = 1.4426950408889634f;
 
 template <int D, int NT>
@@ -635,10 +637,10 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, int cl, cudaStream_
 
 namespace lb {
 // The few-token kernel passes over a sequence's keys once for every 16 rows (new tokens x heads of a group), the tcgen05
-// kernel once for 256. Measured (8 kv heads, bf16, 128 channels, us, few-token / tcgen05): 16 rows 45 / 51 (1 sequence of
-// 32768 keys), 369 / 383 (64 of 8192), 116 / 156 (256 of 500); 32 rows 72 / 51, 694 / 385, 186 / 160. With little work for
-// each block the few-token kernel's shorter start decides: 1 sequence of 2000 keys 18 / 27 at 32 rows, 23 / 27 at 64,
-// 27 / 27 at 128; 300 keys 14 / 18.
+// kernel once for 256. Measured (8 kv heads, 128 channels, us, few-token / tcgen05): 16 rows 46 / 52 (1 sequence of
+// 32768 keys), 351 / 394 (64 of 8192), 134 / 165 (256 of 500); 32 rows 71 / 52, 663 / 398, 230 / 161. With little work for
+// each block the few-token kernel's shorter start decides: 1 sequence of 2000 keys 22 / 27 at 32 rows, 25 / 28 at 64,
+// 30 / 28 at 128; 300 keys 17 / 19.
 constexpr int CHUNK_ROWS = 16;
 constexpr int FEW_BLOCKS = 8;  // 64-key blocks for a thread block of the few-token kernel
 static bool use_chunk(const LbPagedAttnArgs& a) {
