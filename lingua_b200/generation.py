@@ -199,6 +199,15 @@ class LogitControls:
     def __init__(self, cfg: PackedCausalTransformerGeneratorArgs, grammar=None):
         self.repetition, self.presence, self.frequency = cfg.repetition_penalty, cfg.presence_penalty, cfg.frequency_penalty
         self.bias_of, self.allowed_ids, self.grammar = cfg.logit_bias, cfg.allowed_tokens, grammar
+        if not all(map(math.isfinite, (self.repetition, self.presence, self.frequency))) or self.repetition <= 0:
+            raise ValueError("penalties must be finite numbers, repetition_penalty positive")
+        bias = self.bias_of or {}
+        if any(math.isnan(float(b)) or float(b) == math.inf for b in bias.values()):
+            raise ValueError("logit_bias must be finite, or -inf for a token that is never sampled")
+        if self.allowed_ids is not None and len(self.allowed_ids) == 0:
+            raise ValueError("allowed_tokens leaves nothing to sample from")
+        if min((int(t) for t in (*bias, *(self.allowed_ids or ()))), default=0) < 0:
+            raise ValueError("logit_bias and allowed_tokens take token ids, not negative numbers")
 
     def __bool__(self):
         return (self.repetition != 1.0 or self.presence != 0.0 or self.frequency != 0.0 or bool(self.bias_of)
@@ -214,14 +223,19 @@ class LogitControls:
         self.length = self.prompt_len.clone()
         self.bias = self.allowed = None
 
-    def apply(self, logits: torch.Tensor, generated: List[List[int]]) -> torch.Tensor:
-        """logits [n_seqs, vocab] -> what is sampled from."""
+    def apply(self, logits: torch.Tensor, generated: List[List[int]], done: List[bool]) -> torch.Tensor:
+        """logits [n_seqs, vocab] -> what is sampled from. A sequence with no token left to sample is an error, unless it is
+        ``done``: then what is sampled for it is not used."""
         V, dev = logits.shape[1], logits.device
         if self.bias_of and self.bias is None:
+            if max(int(t) for t in self.bias_of) >= V:
+                raise ValueError(f"logit_bias takes token ids below {V}")
             self.bias = torch.zeros(V, device=dev)
             for t, b in self.bias_of.items():
                 self.bias[int(t)] = float(b)
         if self.allowed_ids is not None and self.allowed is None:
+            if max(self.allowed_ids) >= V:
+                raise ValueError(f"allowed_tokens takes token ids below {V}")
             ok = torch.zeros((V + 31) // 32 * 32, dtype=torch.int64)
             ok[torch.tensor(self.allowed_ids, dtype=torch.long)] = 1
             words = (ok.view(-1, 32) << torch.arange(32)).sum(1)
@@ -232,8 +246,16 @@ class LogitControls:
             if mask is not None:
                 mask = mask.to(dev)
                 allowed = mask if allowed is None else mask & allowed
-        return penalize_logits(logits, self.history, self.length, self.prompt_len, self.repetition, self.presence,
-                               self.frequency, self.bias, allowed)
+        z = penalize_logits(logits, self.history, self.length, self.prompt_len, self.repetition, self.presence,
+                            self.frequency, self.bias, allowed)
+        if self.bias is not None or allowed is not None:
+            none_left = torch.isneginf(z.amax(1))
+            rows = torch.nonzero(none_left).view(-1).tolist()
+            if any(not done[i] for i in rows):
+                raise ValueError("logit controls leave nothing to sample from")
+            if rows:
+                z[none_left] = 0.0
+        return z
 
     def took(self, tokens: torch.Tensor) -> None:
         """tokens [n_seqs]: what was sampled."""
@@ -272,7 +294,7 @@ class PackedCausalTransformerGenerator:
     def clear_cache(self):
         for module in self.model.modules():
             if isinstance(module, Attention):
-                if getattr(module, "kv_cache", None) is None:
+                if not isinstance(getattr(module, "kv_cache", None), KVCache):
                     p = next(module.parameters())
                     module.kv_cache = KVCache(self.max_tokens, module.n_kv_heads, module.head_dim, p.dtype,
                                               p.device, self.plan)
@@ -345,16 +367,23 @@ class PackedCausalTransformerGenerator:
         """Cache slots that a prompt and what is generated from it take."""
         return prompt_len + self.max_gen_len
 
-    def _sample(self, logits: torch.Tensor, generated: List[List[int]]) -> torch.Tensor:
+    def _sample(self, logits: torch.Tensor, generated: List[List[int]], done: List[bool]) -> torch.Tensor:
         """logits [1, n_seqs, vocab] of the next token -> tokens [1, n_seqs]."""
         if not self.controls:
             return sample_tokens(logits.clone(), self.temperature, self.top_p, self.top_k)
-        nxt = sample_tokens(self.controls.apply(logits[0], generated).unsqueeze(0), self.temperature, self.top_p, self.top_k)
+        z = self.controls.apply(logits[0], generated, done)
+        nxt = sample_tokens(z.unsqueeze(0), self.temperature, self.top_p, self.top_k)
         self.controls.took(nxt[0])
         return nxt
 
-    @torch.inference_mode()
     def generate(self, prompts: List[str]):
+        try:
+            return self._generate(prompts)
+        finally:  # a model that keeps its cache after an error would attend through it
+            self.release_cache()
+
+    @torch.inference_mode()
+    def _generate(self, prompts: List[str]):
         prompts = [self.tokenizer.encode(p, add_bos=True, add_eos=False) for p in prompts]
         max_seqlen = getattr(self.model, "max_seqlen", self.max_tokens)
         max_prompt_len = self.max_prompt_len or min(max_seqlen - self.max_gen_len, self.max_tokens - self.max_gen_len)
@@ -377,7 +406,7 @@ class PackedCausalTransformerGenerator:
                 last = prompt_logits[:, lengths.cumsum(0) - 1].repeat_interleave(self.samples, dim=1)
                 if self.controls:
                     self.controls.start([p for p in batch for _ in range(self.samples)], self.max_gen_len, last.device)
-                start_token = self._sample(last, generated)
+                start_token = self._sample(last, generated, is_done)
             else:
                 all_tokens = sample_tokens(prompt_logits, self.temperature, self.top_p, self.top_k)
                 start_token = all_tokens[:, lengths.cumsum(0) - 1]
@@ -386,7 +415,7 @@ class PackedCausalTransformerGenerator:
             current = start_token
             for _ in range(1, self.max_gen_len):
                 logits = self.generate_next_token(current)
-                nxt = self._sample(logits, generated)
+                nxt = self._sample(logits, generated, is_done)
                 for i, tok in enumerate(nxt.squeeze(0).tolist()):
                     if not is_done[i]:
                         generated[i].append(tok)
@@ -403,7 +432,6 @@ class PackedCausalTransformerGenerator:
                 y = torch.tensor(p[1:], device=x.device)
                 loglikelihood.append(-TF.cross_entropy(x, y, reduction="none").cpu())
                 greedy.append((x.argmax(dim=-1) == y).cpu())
-        self.release_cache()
         return generation, loglikelihood, greedy
 
 

@@ -240,3 +240,64 @@ def test_generators_refuse_what_they_do_not_do():
     with pytest.raises(CacheFull):
         build_generator(args(page_size=16, max_tokens=16, max_prompt_len=30), model, tok).generate(PROMPTS)
     assert sample_tokens(torch.zeros(1, 2, 4)).shape == (1, 2)
+
+
+def test_controls_that_leave_nothing_to_sample():
+    model, tok = model_of(), ByteTokenizer()
+    nan, inf = float("nan"), float("inf")
+    for kw in (dict(allowed_tokens=[]), dict(allowed_tokens=[-1]), dict(logit_bias={-2: 1.0}), dict(logit_bias={1: nan}),
+               dict(logit_bias={1: inf}), dict(repetition_penalty=0.0), dict(repetition_penalty=inf),
+               dict(presence_penalty=nan), dict(frequency_penalty=-inf)):
+        with pytest.raises(ValueError):
+            build_generator(args(**kw), model, tok)
+    for kw in (dict(allowed_tokens=[3, 258]), dict(logit_bias={300: 1.0}), dict(allowed_tokens=[3], logit_bias={3: -inf})):
+        with pytest.raises(ValueError):
+            build_generator(args(temperature=1.0, **kw), model, tok).generate(PROMPTS[:1])
+    # a grammar that has come to its end allows nothing: no matter for a text that is done, an error for one that goes on
+    def only(tokens):
+        words = [0] * 9
+        for t in tokens:
+            words[t // 32] |= 1 << t % 32
+        return words
+
+    def grammar(out):
+        return torch.tensor([only([ord("a")] if len(out[0]) < 2 else []), only([ord("b")])], dtype=torch.int32)
+
+    for page in (0, 16):
+        gen = build_generator(args(temperature=1.0, page_size=page, until=["aa"]), model, tok)
+        gen.controls.grammar = grammar
+        assert gen.generate(PROMPTS[:2])[0] == ["aa", "b" * 20]
+        gen = build_generator(args(temperature=1.0, page_size=page), model, tok)
+        gen.controls.grammar = grammar
+        with pytest.raises(ValueError):
+            gen.generate(PROMPTS[:2])
+    never = build_generator(args(temperature=1.0, logit_bias={t: -inf for t in range(258) if t != ord("z")}), model, tok)
+    assert never.generate(PROMPTS[:1])[0] == ["z" * 20]
+
+
+def test_an_error_leaves_no_cache_behind():
+    """Generation that fails half way gives the cache back: the model itself and other generators of it work as before."""
+    model, tok = model_of(), ByteTokenizer()
+    ids = torch.tensor([tok.encode(PROMPTS[0], add_bos=True)])
+    want = model(ids)
+    free = build_generator(args(), model, tok).generate(PROMPTS)[0]
+
+    def stop(out):
+        if len(out[0]) == 3:
+            raise RuntimeError("stop")
+
+    for page in (0, 16):
+        gen = build_generator(args(page_size=page), model, tok)
+        gen.controls.grammar = stop
+        with pytest.raises(RuntimeError, match="stop"):
+            gen.generate(PROMPTS)
+        assert torch.equal(model(ids), want)
+        gen.controls.grammar = None
+        assert gen.generate(PROMPTS)[0] == free
+    # caches of the two kinds do not take each other's place
+    paged, flat = build_generator(args(page_size=16), model, tok), build_generator(args(), model, tok)
+    lens = torch.tensor([ids.numel()])
+    with torch.inference_mode():
+        for gen in (paged, flat, paged, flat):
+            assert torch.allclose(gen.prefill(ids, lens), want, atol=1e-4)
+    flat.release_cache()
