@@ -367,6 +367,10 @@ class PackedCausalTransformerGenerator:
         """Cache slots that a prompt and what is generated from it take."""
         return prompt_len + self.max_gen_len
 
+    def prompt_room(self) -> int:
+        """Longest prompt that the cache holds together with what is generated from it."""
+        return self.max_tokens - self.max_gen_len
+
     def _sample(self, logits: torch.Tensor, generated: List[List[int]], done: List[bool]) -> torch.Tensor:
         """logits [1, n_seqs, vocab] of the next token -> tokens [1, n_seqs]."""
         if not self.controls:
@@ -386,7 +390,7 @@ class PackedCausalTransformerGenerator:
     def _generate(self, prompts: List[str]):
         prompts = [self.tokenizer.encode(p, add_bos=True, add_eos=False) for p in prompts]
         max_seqlen = getattr(self.model, "max_seqlen", self.max_tokens)
-        max_prompt_len = self.max_prompt_len or min(max_seqlen - self.max_gen_len, self.max_tokens - self.max_gen_len)
+        max_prompt_len = self.max_prompt_len or min(max_seqlen - self.max_gen_len, self.prompt_room())
         prompts = [p[-max_prompt_len:] for p in prompts]
         padded_lengths = [self.cache_need(len(p)) for p in prompts]
         generation, loglikelihood, greedy = [], [], []

@@ -82,6 +82,15 @@ class PagedCausalTransformerGenerator(PackedCausalTransformerGenerator):
         own = (prompt_len + self.max_gen_len + P - 1) // P - shared
         return (shared + self.samples * own) * P
 
+    def prompt_room(self) -> int:
+        """Longest prompt such that it and all shorter ones fit (rounding to pages makes some shorter ones need more)."""
+        slots, n = max(1, self.max_tokens // self.page_size) * self.page_size, 0
+        while n < self.max_tokens and self.cache_need(n + 1) <= slots:
+            n += 1
+        if n == 0:
+            raise ValueError(f"max_tokens={self.max_tokens} has no room for a prompt and {self.samples} x {self.max_gen_len} new tokens")
+        return n
+
     def clear_cache(self):
         if self.cache is None:
             at, p = self._layers[0], next(self.model.parameters())

@@ -301,3 +301,15 @@ def test_an_error_leaves_no_cache_behind():
         for gen in (paged, flat, paged, flat):
             assert torch.allclose(gen.prefill(ids, lens), want, atol=1e-4)
     flat.release_cache()
+
+
+@pytest.mark.parametrize("samples,max_tokens", [(1, 100), (3, 160), (4, 203)])
+def test_long_prompts_are_cut_to_what_the_cache_holds(samples, max_tokens):
+    model, tok = model_of(), ByteTokenizer()
+    gen = build_generator(args(page_size=16, max_tokens=max_tokens, samples_per_prompt=samples), model, tok)
+    room = gen.prompt_room()
+    assert 0 < room <= max_tokens - 20 and all(gen.cache_need(n) <= max_tokens for n in range(1, room + 1))
+    texts = gen.generate(["x" * n for n in range(room - 18, room + 3)] + ["y" * 300])[0]
+    assert len(texts) == 22 * samples and all(texts)
+    with pytest.raises(ValueError):
+        build_generator(args(page_size=16, max_tokens=16, samples_per_prompt=samples), model, tok).generate(["a"])
