@@ -31,6 +31,19 @@ def _rows(t: Optional[torch.Tensor], dtype: torch.dtype, shape, dev: int) -> boo
                          and (shape[-1] <= 1 or t.stride(-1) == 1))
 
 
+def _torn(out: torch.Tensor, logits: torch.Tensor) -> bool:
+    """Whether ``out`` overlaps the logits without being them: a block would read what another one has written."""
+    a, b = out.data_ptr(), logits.data_ptr()
+    if out.numel() == 0 or (a == b and (out.shape[0] <= 1 or out.stride(0) == logits.stride(0))):
+        return False
+    es, V = out.element_size(), out.shape[1]
+    end = [t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + V) * es for t in (out, logits)]
+    if a >= end[1] or b >= end[0]:
+        return False
+    row = out.stride(0) * es  # rows of one spacing may lie side by side
+    return out.stride(0) != logits.stride(0) or not V * es <= (a - b) % row <= row - V * es
+
+
 def penalize_logits_ref(logits, history, history_len, prompt_len=None, repetition=None, presence=None, frequency=None,
                         bias=None, allowed=None):
     N, V = logits.shape
@@ -67,7 +80,7 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
     frequency     subtracted once per occurrence among the generated tokens
     bias          fp32 [V] or [N, V], added
     allowed       int32 [N, ceil(V / 32)]: bit (t % 32) of word t / 32 clear means token t becomes -inf, whatever its logit
-    out           destination, ``logits`` itself included; a new tensor by default
+    out           destination: ``logits`` itself or memory apart from them; a new tensor by default
 
     The penalties are numbers or fp32 [N] tensors. A row whose mask allows nothing comes out as -inf everywhere."""
     _refuse(logits.dim() != 2, "logits must be [N, V]")
@@ -83,7 +96,7 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
             and _rows(history_len, i32, (N,), dev) and _rows(prompt_len, i32, (N,), dev)
             and (bias is None or _rows(bias, torch.float32, (V,) if bias.dim() == 1 else (N, V), dev))
             and _rows(allowed, i32, (N, (V + 31) // 32), dev)
-            and _rows(out, dt, (N, V), dev) and (out is None or N <= 1 or out.stride(0) >= V) and not _tracked(logits)):
+            and _rows(out, dt, (N, V), dev) and (out is None or ((N <= 1 or out.stride(0) >= V) and not _torn(out, logits))) and not _tracked(logits)):
         # something is unusual: the reference path, or words for what is wrong
         _refuse(history.dim() != 2 or history.shape[0] != N or history.dtype != torch.int64, "history must be int64 [N, L]")
         for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):
@@ -97,6 +110,7 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
         if out is not None:
             _refuse(out.shape != logits.shape or out.dtype != dt, "out must have the logits' shape and dtype")
             _refuse(N > 1 and out.stride(0) < V, "rows of out must not overlap")
+            _refuse(_torn(out, logits), "out must be the logits themselves or not overlap them")
         _refuse(_tracked(logits), "penalize_logits has no gradient")
         if not logits.is_cuda:
             z = penalize_logits_ref(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, allowed)

@@ -133,3 +133,20 @@ def test_penalize_refusals():
             L.penalize_logits(**{**dict(logits=x, history=hist, history_len=hl), **kw})
     out = torch.empty_like(x)
     assert L.penalize_logits(x, hist, hl, out=out) is out
+
+
+def test_penalize_destinations():
+    x, hist, hl, pl, _ = _logits_inputs(3, 40, 6)
+    kw = dict(history=hist, history_len=hl, repetition=1.5, presence=0.5)
+    want = L.penalize_logits(x, **kw)
+    both = torch.zeros(3, 90)
+    both[:, :40] = x
+    left, right = both[:, :40], both[:, 50:]
+    assert torch.equal(L.penalize_logits(left, **kw, out=right), want) and torch.equal(left, x)
+    for bad in (both[:, 1:41], both[:, 39:79], both.view(-1)[90:210].view(3, 40), both.view(-1)[20:140].view(3, 40)):
+        with pytest.raises(ValueError):
+            L.penalize_logits(left, **kw, out=bad)
+    assert torch.equal(L.penalize_logits(left, **kw, out=left), want) and torch.equal(left, want)
+    one = torch.zeros(1, 50)
+    with pytest.raises(ValueError):
+        L.penalize_logits(one[:, :40], hist[:1], hl[:1], out=one[:, 8:48])
