@@ -463,13 +463,13 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         for (int w = 0; w < 4; ++w) {
           const float4 x = *reinterpret_cast<const float4*>(obuf + (w * ROWS + row) * Cfg::OROW + ch);
           o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-          L += sm_m[w][row] == -INFINITY ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);
+          L += sm_l[w][row] == 0.f ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);  // NaN scores leave m at -inf
         }
         if (cl) {  // nobody else reads or writes these four floats of the merge buffer
           *reinterpret_cast<float4*>(obuf + row * Cfg::OROW + ch) = o;
           if (ch == 0) { part_m[row] = M; part_l[row] = L; }
         } else if (whole_item) {
-          const float inv = L > 0.f ? 1.f / L : 0.f;
+          const float inv = L == 0.f ? 0.f : 1.f / L;
           const int gr = row0 + row;
           __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
           *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
         m[p] = -INFINITY;
+        l[p] = 0.f;
         if (p < cl) {
           m[p] = ld_cluster(map_cluster(pm + 4 * row, p));
           l[p] = ld_cluster(map_cluster(pl + 4 * row, p));
@@ -520,13 +521,13 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
       for (int p = 0; p < 8; ++p) M = fmaxf(M, m[p]);
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
-        if (m[p] != -INFINITY) {
+        if (l[p] != 0.f) {
           const float f = exp2f(m[p] - M);
           L += f * l[p];
           o.x += f * x[p].x; o.y += f * x[p].y; o.z += f * x[p].z; o.w += f * x[p].w;
         }
       }
-      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L == 0.f ? 0.f : 1.f / L;
       const int gr = row0 + row;
       __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const LbPagedAtt
       x += sm_o[w][threadIdx.x] * f;
     }
     ((__nv_bfloat16*)a.o)[((long long)(q.q0 + row / G) * a.H + h.y * G + row % G) * D + threadIdx.x] =
-        __float2bfloat16(L > 0.f ? x / L : 0.f);
+        __float2bfloat16(L == 0.f ? 0.f : x / L);  // 0: the row sees no key. NaN stays NaN
   }
 }
 

@@ -7,6 +7,9 @@ which are its last positions. New tokens are packed rows: ``cu_q`` (int32 [n_seq
 ``cu_q=None`` means one token per sequence. Rows that belong to no sequence (behind ``cu_q[-1]``, or with a position below
 zero, as for a sequence with ``kv_len`` 0) are padding: they come out as zeros and leave the cache alone.
 
+What a page holds where no row of its sequence may look is never seen, NaN included. A NaN or infinity among the values that
+one of the call's rows sees may reach the sequence's other rows too, as in a product with a masked matrix of probabilities.
+
 The tables live on the device and may change between replays of a captured graph. A page id outside the pool, or a position
 past the table (or past the rotary table), is skipped and recorded in the status word that ``_lib.check_status`` raises on;
 what the call returns for such a sequence is finite and otherwise unspecified. These are inference operators: no gradients.

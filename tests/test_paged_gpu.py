@@ -313,3 +313,28 @@ def test_offsets_past_32_bits():
     P.copy_pages(pool, last[:3].contiguous(), torch.tensor([0, 5, n_pages - 1], dtype=torch.int32, device=DEV))
     for s, d in zip(last[:3].tolist(), (0, 5, n_pages - 1)):
         assert torch.equal(pool[:, d], pool[:, s])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q,kv", [([1, 1], [100, 40]), ([1], [511]), ([1, 1], [20001, 70]), ([5], [9000]), ([300, 40], [9000, 90])])
+def test_what_is_not_a_number_stays_so(q, kv, D):
+    """A NaN among the scores that a row sees gives NaN, whichever way the row's keys are cut up; other rows are as before."""
+    b = make_batch(q, kv, 8, 2, D, 64, DEV, seed=D + kv[0])
+    one = max(q) == 1
+    ref, mag = attention64(b)
+    tol = attention_tolerance(ref, mag)
+
+    def expect(o, lost):
+        assert torch.equal(torch.isnan(o), lost)
+        assert ((o.double() - ref).abs() <= tol)[~lost].all()
+
+    dirty = dict(b, q=b["q"].clone())
+    dirty["q"][0, 3, 7] = float("nan")
+    lost = torch.zeros(ref.shape, dtype=torch.bool, device=DEV)
+    lost[0, 3] = True
+    expect(attend(dirty, one=one), lost)
+    at = kv[0] - 1 - q[0] // 2  # a key that the first sequence's later rows see
+    b["k_pages"][b["table"][0, at // 64].item(), at % 64, 1, 9] = float("nan")
+    lost = torch.zeros(ref.shape, dtype=torch.bool, device=DEV)
+    lost[q[0] - 1 - q[0] // 2:q[0], 4:] = True
+    expect(attend(b, one=one), lost)
