@@ -119,7 +119,7 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
         _refuse(N > 65535, "too many rows")
         raise ValueError("rows must be contiguous")
     if out is None:
-        out = logits.new_empty((N, V))
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     if N == 0 or V == 0:
         return out
     args = _lib.PENALIZE_ARGS.pack(

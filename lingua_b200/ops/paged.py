@@ -63,23 +63,38 @@ def _aligned(t: torch.Tensor) -> bool:
     return all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
 
 
+def _plain(*strides: int) -> bool:
+    """Strides that need no look at the sizes (that of a dimension of size one may be anything)."""
+    bits = 0
+    for s in strides:
+        bits |= s
+    return not bits & 7 and min(strides) > 0
+
+
 def _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
-    """One pass over the conditions; ``_refuse_cache`` finds the words when one fails."""
+    """One pass over the conditions; ``_refuse_cache`` finds the words when one fails. Returns the sizes and strides that the
+    kernels' argument blocks are made of, read once: (device, T, H, D, n_pages, page, Hkv, n_seqs, cols, stride of a table
+    row, (strides of q), (of k_pages), (of v_pages)), the strides without that of the channels."""
     dev, dt, i32 = q.get_device(), q.dtype, torch.int32
-    if (q.dim() == 3 and k_pages.dim() == 4 and block_table.dim() == 2 and dev >= 0 and dt is torch.bfloat16):
-        n_pages, P, Hkv, D = shape = k_pages.shape
-        n = block_table.shape[0]
-        if (shape == v_pages.shape and q.shape[2] == D and D in HEAD_DIMS and P in PAGE_SIZES and n_pages > 0 and Hkv > 0
-                and q.shape[1] > 0 and q.shape[1] % Hkv == 0 and k_pages.dtype is dt and v_pages.dtype is dt
+    qs, ks, bs = q.shape, k_pages.shape, block_table.shape
+    if len(qs) == 3 and len(ks) == 4 and len(bs) == 2 and dev >= 0 and dt is torch.bfloat16:
+        (T, H, D), (n_pages, P, Hkv, Dk), (n, cols) = qs, ks, bs
+        if (ks == v_pages.shape and Dk == D and D in HEAD_DIMS and P in PAGE_SIZES and n_pages > 0 and Hkv > 0
+                and H > 0 and H % Hkv == 0 and k_pages.dtype is dt and v_pages.dtype is dt
                 and block_table.dtype is i32 and kv_len.dtype is i32 and kv_len.shape == (n,)
-                and k_pages.get_device() == dev and v_pages.get_device() == dev and block_table.get_device() == dev
-                and kv_len.get_device() == dev and kv_len.is_contiguous()
-                and (q.shape[0] == n if cu_q is None else cu_q.dtype is i32 and cu_q.shape == (n + 1,)
+                and dev == k_pages.get_device() == v_pages.get_device() == block_table.get_device() == kv_len.get_device()
+                and kv_len.is_contiguous()
+                and (T == n if cu_q is None else cu_q.dtype is i32 and cu_q.shape == (n + 1,)
                      and cu_q.get_device() == dev and cu_q.is_contiguous())
-                and (block_table.stride(1) == 1 or block_table.shape[1] <= 1) and block_table.shape[1] * P <= MAX_POSITIONS
-                and _aligned(q) and _aligned(k_pages) and _aligned(v_pages) and not _tracked(q, k_pages, v_pages)):
-            return
+                and cols * P <= MAX_POSITIONS and not _tracked(q, k_pages, v_pages)):
+            row, col = block_table.stride()
+            (*q_st, q_c), (*k_st, k_c), (*v_st, v_c) = q.stride(), k_pages.stride(), v_pages.stride()
+            if ((col == 1 or cols <= 1) and q_c == k_c == v_c == 1
+                    and not (q.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr()) & 15
+                    and (_plain(*q_st, *k_st, *v_st) or _aligned(q) and _aligned(k_pages) and _aligned(v_pages))):
+                return dev, T, H, D, n_pages, P, Hkv, n, cols, row, q_st, k_st, v_st
     _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
+    return (dev, *qs, *ks[:3], *bs, block_table.stride(0), q.stride()[:2], k_pages.stride()[:3], v_pages.stride()[:3])
 
 
 def _refuse_cache(q, k_pages, v_pages, block_table, kv_len, cu_q):
@@ -178,10 +193,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
 
     With ``cs`` (rotary table [positions, D / 2, 2], fp32) queries and keys are rotated by their position on the way, as
     ``functional.rope_`` does; k itself is not changed. Two tokens must not share a position of a page."""
-    _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
-    T, H, D = q.shape
-    n_pages, P, Hkv, _ = k_pages.shape
-    dev, dt, shape = q.get_device(), q.dtype, (T, Hkv, D)
+    dev, T, H, D, n_pages, P, Hkv, n, cols, row, q_st, kp_st, vp_st = _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
+    dt, shape = q.dtype, (T, Hkv, D)
     if not (dev >= 0 and k.shape == shape and v.shape == shape and k.dtype is dt and v.dtype is dt and k.get_device() == dev
             and v.get_device() == dev and _aligned(k) and _aligned(v) and not _tracked(k, v)
             and (cs is None or (cs.dtype is torch.float32 and cs.dim() == 3 and cs.shape[1] == D // 2 and cs.shape[2] == 2
@@ -198,16 +211,15 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
         _refuse(cs is not None and cs.data_ptr() % 16 != 0, "cs must be 16-byte aligned")
         _strided(k, "k")
         _strided(v, "v")
-    out = q.new_empty((T, H, D))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if T == 0:
         return out
     args = _lib.PAGED_APPEND_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
         block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
         0 if cs is None else cs.data_ptr(), _status(dev),
-        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], 0 if cs is None else cs.shape[0],
-        block_table.stride(0), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3],
-        *v_pages.stride()[:3])
+        T, n, H, Hkv, D, P, n_pages, cols, 0 if cs is None else cs.shape[0],
+        row, *q_st, *k.stride()[:2], *v.stride()[:2], *kp_st, *vp_st)
     with _on(dev):
         rc = _lib.load().lb_paged_append(args, _lib.stream_ptr())
     _lib.check(rc, "lb_paged_append")
@@ -252,24 +264,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     A token at position p sees the keys j <= p; with ``window`` > 0 of those only j > p - window and the first ``sinks``
     positions. Pages that hold no visible position are not read. ``max_q``: most new tokens of a sequence, used to choose
     the kernel (a wrong value costs speed, not correctness)."""
-    _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
+    dev, T, H, D, n_pages, P, Hkv, n, cols, row, q_st, kp_st, vp_st = _check_cache(q, k_pages, v_pages, block_table, kv_len, cu_q)
     _refuse(window < 0 or sinks < 0, "window and sinks must not be negative")
     window, sinks = window if window < MAX_POSITIONS else 0, min(sinks, MAX_POSITIONS)  # no position is further away
-    T, H, D = q.shape
-    n_pages, P, Hkv, _ = k_pages.shape
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     _refuse(not scale >= 0.0, "scale must not be negative")
     if not q.is_cuda:
         return paged_attention_ref(q, k_pages, v_pages, block_table, kv_len, cu_q, scale, window, sinks)
-    out = q.new_empty((T, H, D))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if T == 0:
         return out
-    dev = q.get_device()
     args = _lib.PAGED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
         0 if cu_q is None else cu_q.data_ptr(), _status(dev),
-        T, block_table.shape[0], H, Hkv, D, P, n_pages, block_table.shape[1], window, sinks, min(max_q, MAX_POSITIONS), scale,
-        block_table.stride(0), *q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
+        T, n, H, Hkv, D, P, n_pages, cols, window, sinks, min(max_q, MAX_POSITIONS), scale, row, *q_st, *kp_st, *vp_st)
     lib = _lib.load()
     with _on(dev):
         need = lib.lb_paged_attention_workspace(args)

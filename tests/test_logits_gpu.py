@@ -90,3 +90,19 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError):
         penalize_logits(X, Hh, Hl, out=torch.empty(1, 64, device=DEV).expand(2, 64))
     assert penalize_logits(X[:0], Hh[:0], Hl[:0]).shape == (0, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_destinations(dtype):
+    both = torch.randn(3, 2 * 5000 + 24, device=DEV).to(dtype)
+    left, right = both[:, :5000], both[:, 5008:10008]
+    hist = torch.randint(0, 5000, (3, 50), device=DEV)
+    kw = dict(history=hist, history_len=torch.tensor([50, 0, 7], dtype=torch.int32, device=DEV), repetition=1.5, frequency=0.25)
+    want = penalize_logits(left, **kw)
+    penalize_logits(left, **kw, out=right)
+    assert torch.equal(right, want)
+    for bad in (both[:, 8:5008], both[:, 4992:9992], both.view(-1)[8000:23000].view(3, 5000)):
+        with pytest.raises(ValueError):
+            penalize_logits(left, **kw, out=bad)
+    penalize_logits(left, **kw, out=left)
+    assert torch.equal(left, want)

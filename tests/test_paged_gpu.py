@@ -338,3 +338,30 @@ def test_what_is_not_a_number_stays_so(q, kv, D):
     lost = torch.zeros(ref.shape, dtype=torch.bool, device=DEV)
     lost[q[0] - 1 - q[0] // 2:q[0], 4:] = True
     expect(attend(b, one=one), lost)
+
+
+def test_two_graphs_at_once():
+    """Graphs of calls that cut sequences up, replayed on two streams at the same time: neither disturbs the other's parts."""
+    cases = [([1, 1, 1], [30000, 17, 9000]), ([300, 1], [9000, 4000])]
+    graphs, outs, want = [], [], []
+    for q, kv in cases:
+        b = make_batch(q, kv, 8, 2, 128, 64, DEV, seed=kv[0])
+        one = max(q) == 1
+        want.append(attend(b, one=one))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = attend(b, one=one)
+        graphs.append((g, b))  # the inputs stay where the graph reads them
+        outs.append(o)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    _lib.check_status()
