@@ -4,7 +4,7 @@
 // the ones with j > p - W or j < sinks. A row that sees no key (a padding row, an empty sequence) gives zeros.
 //
 // Bound by reading every visible key and value row once (2 D 2 bytes per key and kv head; G = H / Hkv query heads share
-// them). Measured: 64 sequences of up to 8192 keys, 32 / 8 heads (1.2 GB) 195 us, 6.1 TB/s; one of 131072 keys 91 us, 5.9 TB/s;
+// them). Measured: 64 sequences of up to 8192 keys, 32 / 8 heads (1.2 GB) 188 us, 6.4 TB/s; one of 131072 keys 90 us, 6.0 TB/s;
 // one of 511 keys, 16 heads, 6.6 us (in a graph). Layout of the work:
 //  * An item is (sequence, kv head, 8 or 16 rows), the rows being (token, head of the group) pairs, so that one pass over
 //    the keys serves the whole group. The products are m16n8k16 with the KEYS on the 16 side and the rows on the 8 side,
@@ -19,7 +19,8 @@
 //    clusters: up to 8 blocks share an item and join their parts through distributed shared memory, in one launch.
 //  * The four warps of a block take 16 keys of a 64-key block each and meet only at the end of an item. Every warp
 //    keeps its own ring of 16-key stages in shared memory, filled by TMA (boxes of 16 keys x 64 channels, 128-byte
-//    swizzle), so a stage is waited for and given back by one warp alone.
+//    swizzle), so a stage is waited for and given back by one warp alone. The join at the end of an item takes one stage of
+//    each ring (two for 16 rows); the others fill with the next item's first blocks meanwhile (batch below 196 -> 188 us).
 //  * ldmatrix reads both operands in place, the values transposed; the swizzle makes its eight rows fall into different
 //    banks. P^T is turned from the layout of a result to that of an operand by movmatrix.
 //  * Keys that no row may see, and pages that are not there, never contribute: scores are replaced (not added to), and
@@ -46,6 +47,7 @@ struct DecCfg {
   static constexpr int NST = D == 128 ? 3 : 6;
   static constexpr int SMEM = 4 * NST * STAGE + 1024;  // 97 KB: two blocks per SM
   static constexpr int OROW = D + 4;                // padded row of the merge buffer (floats)
+  static_assert(8 * OROW * 4 <= STAGE && NT < NST, "a stage holds a row tile of the merge buffer");
   static constexpr int SLOT = ROWS * D + 2 * ROWS;  // floats of one partial result
 };
 
@@ -122,6 +124,12 @@ __device__ __forceinline__ DecSeq dec_seq(const LbPagedAttnArgs& a, int s, bool 
   r.rt = (int)((rows + ROWS - 1) / ROWS);
   return r;
 }
+
+// A block's part of an item: kv head, row tile and 64-key blocks [b0, b1) of a sequence.
+struct DecPiece {
+  int seq, hk, rt, b0, b1;
+  DecSeq q;
+};
 
 struct DecWork {  // found by one thread, read by the block
   int seq;           // sequence of this block's first unit
@@ -221,7 +229,6 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   __syncthreads();
   if (u0 >= u1 && !cl) return;
 
-  float* obuf = reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)));  // the ring, once an item's blocks are done
   const uint32_t ring = dyn0 + warp * (Cfg::NST * Cfg::STAGE);
   const uint32_t bars = smem_u32(&full[warp][0]);
   uint32_t parity = 0;  // bit st: phase the next wait on stage st completes
@@ -238,259 +245,295 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
   }
   const float sl2 = a.scale * DEC_LOG2E;
   const int page_log = __ffs(a.page) - 1;
-  long long left = u1 - u0;
-  int seq = work.seq;
-  long long offset = work.offset;
-  for (; left > 0 && seq < a.n_seqs; ++seq, offset = 0) {
-    const DecSeq q = dec_seq<ROWS>(a, seq, false);
-    const int item_units = split ? q.nb : 1;
-    const long long n_items = (long long)a.Hkv * q.rt;
-    for (long long item = div_nonneg(offset, item_units); left > 0 && item < n_items; ++item) {
-      const int hk = (int)div_nonneg(item, q.rt), rt = (int)(item - (long long)hk * q.rt);
-      const int b0 = split ? (int)(offset - item * item_units > 0 ? offset - item * item_units : 0) : 0;
-      const int b1 = split ? (int)min((long long)q.nb, b0 + left) : q.nb;
-      left -= split ? b1 - b0 : 1;
+  // pieces of this block's share, one after the other
+  long long left = u1 - u0, item = 0, n_items = 0;
+  int first = 0;  // key block that the next piece begins with
+  DecPiece nxt;
+  nxt.seq = work.seq;
+  auto enter = [&]() {
+    nxt.q = dec_seq<ROWS>(a, nxt.seq, false);
+    n_items = (long long)a.Hkv * nxt.q.rt;
+  };
+  auto fetch = [&]() {
+    while (left > 0) {
+      if (item < n_items) {
+        nxt.hk = (int)div_nonneg(item, nxt.q.rt);
+        nxt.rt = (int)(item - (long long)nxt.hk * nxt.q.rt);
+        nxt.b0 = first;
+        nxt.b1 = split ? (int)min((long long)nxt.q.nb, first + left) : nxt.q.nb;
+        left -= split ? nxt.b1 - nxt.b0 : 1;
+        first = 0;
+        ++item;
+        return true;
+      }
+      if (++nxt.seq >= a.n_seqs) return false;
+      item = 0;
+      enter();
+    }
+    return false;
+  };
+  enter();
+  item = div_nonneg(work.offset, split ? nxt.q.nb : 1);
+  if (split) first = (int)(work.offset - item * nxt.q.nb);
 
-      // ---- Q^T fragments: lane (r, c) holds channels 16 k + 2 c, + 1, + 8, + 9 of row 8 t + r
-      const int row0 = rt * ROWS;
-      const int n_rows = min(ROWS, q.nq * G - row0);
-      uint32_t qf[D / 16][NT][2];
-      long long pos[NT][2];  // of rows 8 t + 2 c, + 1
+  // ---- requests: pages of a piece's next 32 + 32 blocks, one per lane
+  int pg = -1, pg_next = -1, filled = 0;
+  auto key_of = [&](const DecPiece& w, int b) { return (b < w.q.sb ? b : b - w.q.sb + w.q.wb) * DEC_BLOCK + warp * 16; };
+  auto page_of = [&](const DecPiece& w, int b) {
+    const int k = key_of(w, b);
+    return b < w.b1 && k < w.q.end ? __ldg(a.table + (long long)w.seq * a.table_stride + (k >> page_log)) : -1;
+  };
+  auto issue = [&](const DecPiece& w, int b, int st) {
+    const int rel = b - w.b0;
+    if ((rel & 31) == 0 && rel) pg = pg_next;
+    if ((rel & 31) == 16) pg_next = page_of(w, b + 16 + lane);
+    int page = __shfl_sync(0xFFFFFFFFu, pg, rel & 31);
+    if (lane == 0) {
+      const int kb = key_of(w, b), off = kb & (a.page - 1);
+      // 16 keys that no row sees are requested outside the pool, where TMA fills with zeros and reads nothing (with a window
+      // of 1024 and the first 4 keys that is a tenth of the bytes: 48 sequences of 32 heads 138 -> 130 us). A visible key
+      // without a page is an error.
+      const bool seen = kb < w.q.end && (kb + 16 > w.q.wlo || kb < a.sinks);
+      if (!seen) page = a.n_pages;
+      if (page < 0 || page >= a.n_pages) {
+        if (seen && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
+        page = a.n_pages;
+      }
+      const uint32_t bar = bars + 8 * st, dst = ring + st * Cfg::STAGE;
+      mbar_arrive_expect_tx(bar, Cfg::STAGE);
+#pragma unroll
+      for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + g * Cfg::BOX, &tk, bar, 64 * g, off, w.hk, page);
+#pragma unroll
+      for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + (Cfg::VG + g) * Cfg::BOX, &tv, bar, 64 * g, off, w.hk, page);
+    }
+  };
+  auto wrap = [](int st) { return st >= Cfg::NST ? st - Cfg::NST : st; };
+  // the first blocks of the next piece, until n stages are filled (all are free once a piece's blocks have been read)
+  auto fill = [&](int n) {
+#pragma unroll 1
+    for (; filled < min(nxt.b1 - nxt.b0, n); ++filled) issue(nxt, nxt.b0 + filled, wrap(head + filled));
+  };
+
+  bool have = fetch();
+  if (have) pg = page_of(nxt, nxt.b0 + lane);
+  while (have) {
+    const DecPiece w = nxt;
+    const DecSeq& q = w.q;
+    const int hk = w.hk, b0 = w.b0, b1 = w.b1;
+
+    // ---- Q^T fragments: lane (r, c) holds channels 16 k + 2 c, + 1, + 8, + 9 of row 8 t + r
+    const int row0 = w.rt * ROWS;
+    const int n_rows = min(ROWS, q.nq * G - row0);
+    uint32_t qf[D / 16][NT][2];
+    long long pos[NT][2];  // of rows 8 t + 2 c, + 1
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = row0 + 8 * t + r;
+      const bool live = 8 * t + r < n_rows;
+      const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (long long)(q.q0 + row / G) * a.q_st +
+                                (long long)(hk * G + row % G) * a.q_sh + 2 * c;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][t][0] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
+        qf[k][t][1] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pos[t][i] = 8 * t + 2 * c + i < n_rows ? q.pos0 + (row0 + 8 * t + 2 * c + i) / G : -1;
+    }
+
+    fill(Cfg::NST);  // of what the previous piece's end has left
+    filled = 0;
+
+    // rows 8 t + 2 c + i: maximum, sum, and O^T: acc[j][t][2 h + i] is channel 16 j + 8 h + r
+    float m[NT][2], l[NT][2];
+    float acc[D / 16][NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { m[t][i] = -INFINITY; l[t][i] = 0.f; }
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][t][i] = 0.f;
+    }
+
+    int prev = head;
+    for (int b = b0; alive && b < b1; ++b) {
+      alive = mbar_wait(bars + 8 * head, (parity >> head) & 1, &abort_flag, a.status, 0x46);
+      alive = __all_sync(0xFFFFFFFFu, alive);
+      if (!alive) break;
+      parity ^= 1u << head;
+      const uint32_t kbox = ring + head * Cfg::STAGE, vbox = kbox + Cfg::VG * Cfg::BOX;
+      // scores: two accumulators for each row tile, so that chains of dependent products are half as long
+      float s[NT][4], s2[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] = s2[t][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t kf[4];
+        ldmatrix_x4(kf, kbox + (k >> 2) * Cfg::BOX + k_off[k & 3]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816(k & 1 ? s2[t] : s[t], kf, qf[k][t][0], qf[k][t][1]);
+      }
+      // what follows needs time until the scores are there: refill the stage of the previous block, read the values
+      if (b > b0 && b + Cfg::NST - 1 < b1) issue(w, b + Cfg::NST - 1, prev);
+      uint32_t vf[D / 16][4];
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) ldmatrix_x4_trans(vf[j], vbox + (j >> 2) * Cfg::BOX + v_off[j & 3]);
+      // in units of log 2; s[t][2 h + i]: key kb + r + 8 h, row 8 t + 2 c + i
+      const int kb = key_of(w, b);
+      const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
+      bool grow = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int row = row0 + 8 * t + r;
-        const bool live = 8 * t + r < n_rows;
-        const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (long long)(q.q0 + row / G) * a.q_st +
-                                  (long long)(hk * G + row % G) * a.q_sh + 2 * c;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qf[k][t][0] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
-          qf[k][t][1] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          pos[t][i] = 8 * t + 2 * c + i < n_rows ? q.pos0 + (row0 + 8 * t + 2 * c + i) / G : -1;
-      }
-
-      // ---- pages of this warp's next 32 + 32 blocks, one per lane
-      const int* trow = a.table + (long long)seq * a.table_stride;
-      auto key_of = [&](int b) { return (b < q.sb ? b : b - q.sb + q.wb) * DEC_BLOCK + warp * 16; };
-      auto page_of = [&](int b) {
-        const int k = key_of(b);
-        return b < b1 && k < q.end ? __ldg(trow + (k >> page_log)) : -1;
-      };
-      int pg = page_of(b0 + lane), pg_next = -1;
-      auto issue = [&](int b, int st) {
-        const int rel = b - b0;
-        if ((rel & 31) == 0 && rel) pg = pg_next;
-        if ((rel & 31) == 16) pg_next = page_of(b + 16 + lane);
-        int page = __shfl_sync(0xFFFFFFFFu, pg, rel & 31);
-        if (lane == 0) {
-          const int kb = key_of(b), off = kb & (a.page - 1);
-          if (page < 0 || page >= a.n_pages) {
-            // hidden keys need no page; a visible key without one is an error. Outside the pool TMA fills with zeros.
-            const bool seen = kb < q.end && (kb + 16 > q.wlo || kb < a.sinks);
-            if (seen && a.status) atomicOr(a.status, ST_BAD_ARG | 0x44u);
-            page = a.n_pages;
+        for (int x = 0; x < 4; ++x) {
+          s[t][x] = (s[t][x] + s2[t][x]) * sl2;
+          if (!whole) {
+            const int j = kb + r + 8 * (x >> 1);
+            const long long p = pos[t][x & 1];
+            if (j > p || j >= q.end || (a.window > 0 && j <= p - a.window && j >= a.sinks)) s[t][x] = -INFINITY;
           }
-          const uint32_t bar = bars + 8 * st, dst = ring + st * Cfg::STAGE;
-          mbar_arrive_expect_tx(bar, Cfg::STAGE);
-#pragma unroll
-          for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + g * Cfg::BOX, &tk, bar, 64 * g, off, hk, page);
-#pragma unroll
-          for (int g = 0; g < Cfg::VG; ++g) tma_load_4d(dst + (Cfg::VG + g) * Cfg::BOX, &tv, bar, 64 * g, off, hk, page);
         }
-      };
-
-      // rows 8 t + 2 c + i: maximum, sum, and O^T: acc[j][t][2 h + i] is channel 16 j + 8 h + r
-      float m[NT][2], l[NT][2];
-      float acc[D / 16][NT][4];
+        // the running maximum only moves when it would be exceeded by more than 2^8 (probabilities stay below 2^8)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { m[t][i] = -INFINITY; l[t][i] = 0.f; }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][t][i] = 0.f;
+        for (int i = 0; i < 2; ++i) grow |= fmaxf(s[t][i], s[t][2 + i]) > m[t][i] + 8.f;
       }
-
-      auto next = [](int st) { return st + 1 == Cfg::NST ? 0 : st + 1; };
-      int fill = head, prev = head;
-      for (int b = b0; b < min(b1, b0 + Cfg::NST); ++b) {
-        issue(b, fill);
-        fill = next(fill);
-      }
-      for (int b = b0; alive && b < b1; ++b) {
-        alive = mbar_wait(bars + 8 * head, (parity >> head) & 1, &abort_flag, a.status, 0x46);
-        alive = __all_sync(0xFFFFFFFFu, alive);
-        if (!alive) break;
-        parity ^= 1u << head;
-        const uint32_t kbox = ring + head * Cfg::STAGE, vbox = kbox + Cfg::VG * Cfg::BOX;
-        // scores: two accumulators for each row tile, so that chains of dependent products are half as long
-        float s[NT][4], s2[NT][4];
+      if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][i] = s2[t][i] = 0.f;
+          for (int i = 0; i < 2; ++i) {
+            float mx = fmaxf(s[t][i], s[t][2 + i]);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          uint32_t kf[4];
-          ldmatrix_x4(kf, kbox + (k >> 2) * Cfg::BOX + k_off[k & 3]);
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            if (mx > m[t][i]) {
+              const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - mx);
+              m[t][i] = mx;
+              l[t][i] *= f;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(k & 1 ? s2[t] : s[t], kf, qf[k][t][0], qf[k][t][1]);
-        }
-        // what follows needs time until the scores are there: refill the stage of the previous block, read the values
-        if (b > b0 && b + Cfg::NST - 1 < b1) issue(b + Cfg::NST - 1, prev);
-        uint32_t vf[D / 16][4];
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) ldmatrix_x4_trans(vf[j], vbox + (j >> 2) * Cfg::BOX + v_off[j & 3]);
-        // in units of log 2; s[t][2 h + i]: key kb + r + 8 h, row 8 t + 2 c + i
-        const int kb = key_of(b);
-        const bool whole = kb + 16 <= q.end - (q.nq - 1) && (kb > q.end - 1 - a.window || a.window <= 0 || kb + 16 <= a.sinks);
-        bool grow = false;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[t][x] = (s[t][x] + s2[t][x]) * sl2;
-            if (!whole) {
-              const int j = kb + r + 8 * (x >> 1);
-              const long long p = pos[t][x & 1];
-              if (j > p || j >= q.end || (a.window > 0 && j <= p - a.window && j >= a.sinks)) s[t][x] = -INFINITY;
+              for (int j = 0; j < D / 16; ++j) { acc[j][t][i] *= f; acc[j][t][2 + i] *= f; }
             }
           }
-          // the running maximum only moves when it would be exceeded by more than 2^8 (probabilities stay below 2^8)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) grow |= fmaxf(s[t][i], s[t][2 + i]) > m[t][i] + 8.f;
-        }
-        if (__any_sync(0xFFFFFFFFu, grow)) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float mx = fmaxf(s[t][i], s[t][2 + i]);
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-              if (mx > m[t][i]) {
-                const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - mx);
-                m[t][i] = mx;
-                l[t][i] *= f;
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) { acc[j][t][i] *= f; acc[j][t][2 + i] *= f; }
-              }
-            }
-        }
-        // probabilities enter the second product in bf16 (half a step, 2^-8 of each); their sum is taken before that
-        uint32_t pt[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p0 = exp2f(s[t][2 * h] - m0), p1 = exp2f(s[t][2 * h + 1] - m1);
-            l[t][0] += p0;
-            l[t][1] += p1;
-            pt[t][h] = movmatrix_trans(pack_bf16(p0, p1));
-          }
-        }
-        uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // keys kb + 2 c, + 1 and those 8 further: which are not hidden
-        if (!whole) {
-          keep0 = keep1 = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = kb + 2 * c + (i & 1) + 8 * (i >> 1);
-            const uint32_t bits = j < q.end && (j >= q.wlo || j < a.sinks) ? 0xFFFFu << (16 * (i & 1)) : 0u;
-            if (i < 2) keep0 |= bits; else keep1 |= bits;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          if (!whole) { vf[j][0] &= keep0; vf[j][1] &= keep0; vf[j][2] &= keep1; vf[j][3] &= keep1; }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(acc[j][t], vf[j], pt[t][0], pt[t][1]);
-        }
-        __syncwarp();  // every lane's pieces are in registers (the products needed them): the stage can be filled again
-        prev = head;
-        head = next(head);
       }
-      // a wait ran out (recorded in the status word): copies in flight land before shared memory is given up
-      if (!alive) {
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-      }
-
-      // ---- join the four warps
+      // probabilities enter the second product in bf16 (half a step, 2^-8 of each); their sum is taken before that
+      uint32_t pt[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], o);
-          if (r == 0) { sm_m[warp][8 * t + 2 * c + i] = m[t][i]; sm_l[warp][8 * t + 2 * c + i] = l[t][i]; }
-        }
-      __syncthreads();
-      if (abort_flag) {  // read by all after the same barrier
-        if (!cl) return;
-        left = 0;  // the other blocks of the cluster are met below; this one has nothing to add
-        break;
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = 8 * t + 2 * c + i;
-          if (row < n_rows) {
-            const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
-            const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - M);
-            float* dst = obuf + (warp * ROWS + row) * Cfg::OROW + r;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-              dst[16 * j] = acc[j][t][i] * f;
-              dst[16 * j + 8] = acc[j][t][2 + i] * f;
-            }
-          }
-        }
-      __syncthreads();
-      const bool whole_item = b0 == 0 && b1 == q.nb;
-      float* slot = whole_item || cl ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
-      for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
-        const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
-        const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float L = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(obuf + (w * ROWS + row) * Cfg::OROW + ch);
-          o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-          L += sm_l[w][row] == 0.f ? 0.f : sm_l[w][row] * exp2f(sm_m[w][row] - M);  // NaN scores leave m at -inf
-        }
-        if (cl) {  // nobody else reads or writes these four floats of the merge buffer
-          *reinterpret_cast<float4*>(obuf + row * Cfg::OROW + ch) = o;
-          if (ch == 0) { part_m[row] = M; part_l[row] = L; }
-        } else if (whole_item) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          const int gr = row0 + row;
-          __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
-          *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-        } else {
-          *reinterpret_cast<float4*>(slot + row * D + ch) = o;
-          if (ch == 0) { slot[ROWS * D + row] = M; slot[ROWS * D + ROWS + row] = L; }
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = exp2f(s[t][2 * h] - m0), p1 = exp2f(s[t][2 * h + 1] - m1);
+          l[t][0] += p0;
+          l[t][1] += p1;
+          pt[t][h] = movmatrix_trans(pack_bf16(p0, p1));
         }
       }
-      if (cl) break;
-      if (!whole_item && b0 == 0 && threadIdx.x == 0) {
-        // units [u1 - (b1 - b0), + nb) hold this item: find the block its last unit belongs to
-        const long long end_unit = u1 - (b1 - b0) + q.nb - 1;
-        // share of unit u: the largest i with total * i / n_blocks <= u
-        long long i = div_nonneg(end_unit * n_blocks, total);
-        while (i + 1 < n_blocks && share(i + 1) <= end_unit) ++i;
-        while (i > 0 && share(i) > end_unit) --i;
-        hdr[blockIdx.x] = make_int4(seq, hk, rt, (int)(i - blockIdx.x + 1));
+      uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // keys kb + 2 c, + 1 and those 8 further: which are not hidden
+      if (!whole) {
+        keep0 = keep1 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = kb + 2 * c + (i & 1) + 8 * (i >> 1);
+          const uint32_t bits = j < q.end && (j >= q.wlo || j < a.sinks) ? 0xFFFFu << (16 * (i & 1)) : 0u;
+          if (i < 2) keep0 |= bits; else keep1 |= bits;
+        }
       }
-      fence_proxy_async_smem();  // the merge buffer becomes the ring again: ordinary accesses before TMA writes
-      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        if (!whole) { vf[j][0] &= keep0; vf[j][1] &= keep0; vf[j][2] &= keep1; vf[j][3] &= keep1; }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816(acc[j][t], vf[j], pt[t][0], pt[t][1]);
+      }
+      __syncwarp();  // every lane's pieces are in registers (the products needed them): the stage can be filled again
+      prev = head;
+      head = wrap(head + 1);
     }
+    // ---- join the four warps. The last NT stages of each ring, counted from where the next piece begins, hold its partial
+    // output; the others take the next piece's first blocks meanwhile.
+    have = left > 0 && fetch();
+    if (have && alive) {
+      pg = page_of(nxt, nxt.b0 + lane);
+      fill(Cfg::NST - NT);
+    }
+    auto obuf = [&](int of, int row) {  // of a cluster's block: where its neighbours know it to be
+      const int st = cl ? row >> 3 : wrap(head + Cfg::NST - 1 - (row >> 3));
+      return reinterpret_cast<float*>(dyn + (dyn0 - smem_u32(dyn)) + (of * Cfg::NST + st) * Cfg::STAGE) + (row & 7) * Cfg::OROW;
+    };
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], o);
+        if (r == 0) { sm_m[warp][8 * t + 2 * c + i] = m[t][i]; sm_l[warp][8 * t + 2 * c + i] = l[t][i]; }
+      }
+    __syncthreads();
+    if (abort_flag) {  // a wait ran out (recorded in the status word); read by all after the same barrier
+      // copies in flight land before shared memory is given up
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      if (!cl) return;
+      break;  // the other blocks of the cluster are met below; this one has nothing to add
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 8 * t + 2 * c + i;
+        if (row < n_rows) {
+          const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+          const float f = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - M);
+          float* dst = obuf(warp, row) + r;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            dst[16 * j] = acc[j][t][i] * f;
+            dst[16 * j + 8] = acc[j][t][2 + i] * f;
+          }
+        }
+      }
+    __syncthreads();
+    const bool whole_item = b0 == 0 && b1 == q.nb;
+    float* slot = whole_item || cl ? nullptr : ws + (long long)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * Cfg::SLOT;
+    for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
+      const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
+      const float M = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll
+      for (int of = 0; of < 4; ++of) {
+        const float4 x = *reinterpret_cast<const float4*>(obuf(of, row) + ch);
+        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        L += sm_l[of][row] == 0.f ? 0.f : sm_l[of][row] * exp2f(sm_m[of][row] - M);  // NaN scores leave m at -inf
+      }
+      if (cl) {  // nobody else reads or writes these four floats of the merge buffer
+        *reinterpret_cast<float4*>(obuf(0, row) + ch) = o;
+        if (ch == 0) { part_m[row] = M; part_l[row] = L; }
+      } else if (whole_item) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int gr = row0 + row;
+        __nv_bfloat16* op = (__nv_bfloat16*)a.o + ((long long)(q.q0 + gr / G) * a.H + hk * G + gr % G) * D + ch;
+        *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(slot + row * D + ch) = o;
+        if (ch == 0) { slot[ROWS * D + row] = M; slot[ROWS * D + ROWS + row] = L; }
+      }
+    }
+    if (cl) break;
+    if (!whole_item && b0 == 0 && threadIdx.x == 0) {
+      // units [u1 - (b1 - b0), + nb) hold this item: find the block its last unit belongs to
+      const long long end_unit = u1 - (b1 - b0) + q.nb - 1;
+      // share of unit u: the largest i with total * i / n_blocks <= u
+      long long i = div_nonneg(end_unit * n_blocks, total);
+      while (i + 1 < n_blocks && share(i + 1) <= end_unit) ++i;
+      while (i > 0 && share(i) > end_unit) --i;
+      hdr[blockIdx.x] = make_int4(w.seq, hk, w.rt, (int)(i - blockIdx.x + 1));
+    }
+    fence_proxy_async_smem();  // the merge buffer becomes the ring again: ordinary accesses before TMA writes
+    __syncthreads();
   }
   if (!cl) return;
 
@@ -501,7 +544,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
     const DecSeq q = dec_seq<ROWS>(a, item / per_seq, false);
     const int hk = (item % per_seq) / q.rt, row0 = (item % per_seq) % q.rt * ROWS;
     const int n_rows = min(ROWS, q.nq * G - row0);
-    const uint32_t pm = smem_u32(part_m), pl = smem_u32(part_l), po = smem_u32(obuf);
+    const uint32_t pm = smem_u32(part_m), pl = smem_u32(part_l);
     for (int i = threadIdx.x + 128 * rank; i < n_rows * (D / 4); i += 128 * cl) {
       const int row = i / (D / 4), ch = (i % (D / 4)) * 4;
       // all parts' loads in flight at once; the buffer of a part that saw no key may hold anything
@@ -514,7 +557,7 @@ __global__ void __launch_bounds__(128, 2) paged_decode_kernel(const __grid_const
         if (p < cl) {
           m[p] = ld_cluster(map_cluster(pm + 4 * row, p));
           l[p] = ld_cluster(map_cluster(pl + 4 * row, p));
-          x[p] = ld_cluster4(map_cluster(po + 4 * (row * Cfg::OROW + ch), p));
+          x[p] = ld_cluster4(map_cluster(dyn0 + (row >> 3) * Cfg::STAGE + 4 * ((row & 7) * Cfg::OROW + ch), p));
         }
       }
 #pragma unroll

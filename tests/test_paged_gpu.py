@@ -365,3 +365,18 @@ def test_two_graphs_at_once():
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
     _lib.check_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(8, 8), (24, 2)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (130, 3)])
+def test_many_items_a_block(H, Hkv, D, window, sinks):
+    """More items than blocks of the grid, of one to forty key blocks: an item's first keys arrive while the one before is joined."""
+    g = torch.Generator().manual_seed(D + H)
+    kv = torch.randint(0, 700, (160,), generator=g).tolist() + [2500, 64, 65, 0, 1, 2560]
+    b = make_batch([1] * len(kv), kv, H, Hkv, D, 32, DEV, seed=H, release=(window, sinks) if window else None)
+    o = attend(b, one=True, window=window, sinks=sinks)
+    check(o, b, window, sinks)
+    assert torch.equal(o, attend(b, one=True, window=window, sinks=sinks))
+    b = make_batch([1] * 200, [40 + i % 200 for i in range(200)], H, Hkv, D, 32, DEV, seed=H)  # items that are not cut up
+    check(attend(b, one=True), b)
