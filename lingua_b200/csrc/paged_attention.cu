@@ -33,8 +33,8 @@
 namespace lb {
 
 constexpr int DEC_BLOCK = 64;       // keys per block: 16 for each warp
-// Items of up to so many blocks are not cut up: 256 keys 7.2 us whole, 7.9 us cut up; 511 keys 10.1 / 7.7 us, 6.5 us by clusters
-// (one sequence, 16 heads, in a graph).
+// Items of up to so many blocks are not cut up into shares that a second kernel joins: 256 keys 7.4 us whole,
+// 300 keys 8.4 us whole and 8.0 us cut up, 511 keys 10.6 / 8.0 (one sequence, 16 heads, in a graph).
 constexpr int NOSPLIT_BLOCKS = 4;
 constexpr float DEC_LOG2E = 1.4426950408889634f;
 
@@ -682,10 +682,10 @@ static int launch_decode(const LbPagedAttnArgs& a, void* ws, int cl, cudaStream_
 
 namespace lb {
 // The few-token kernel passes over a sequence's keys once for every 16 rows (new tokens x heads of a group), the tcgen05
-// kernel once for 256. Measured (8 kv heads, 128 channels, us, few-token / tcgen05): 16 rows 46 / 52 (1 sequence of
-// 32768 keys), 351 / 394 (64 of 8192), 134 / 165 (256 of 500); 32 rows 71 / 52, 663 / 398, 230 / 161. With little work for
-// each block the few-token kernel's shorter start decides: 1 sequence of 2000 keys 22 / 27 at 32 rows, 25 / 28 at 64,
-// 30 / 28 at 128; 300 keys 17 / 19.
+// kernel once for 256. Measured (8 kv heads, 128 channels, us in a graph, few-token / tcgen05): 16 rows 34 / 42 (1 sequence
+// of 32768 keys), 331 / 365 (64 of 8192), 105 / 149 (256 of 500); 32 rows 52 / 41, 629 / 367, 180 / 150. With little work for
+// each block the few-token kernel's shorter start decides: 1 sequence of 2000 keys 14 / 20 at 32 rows, 20 / 20 at 64,
+// 23 / 21 at 128; 300 keys 12 / 15.
 constexpr int CHUNK_ROWS = 16;
 constexpr int FEW_BLOCKS = 8;  // 64-key blocks for a thread block of the few-token kernel
 static bool use_chunk(const LbPagedAttnArgs& a) {
@@ -706,14 +706,16 @@ static long long most_blocks(const LbPagedAttnArgs& a) {
 }
 // Blocks of a cluster that share an item; 0: no clusters. For one token per sequence, and as long as a block of the
 // cluster has no more than FEW_BLOCKS key blocks and the clusters fit the GPU side by side; beyond that equal shares of
-// everything are worth the second launch.
+// everything are worth the second launch. As many blocks as key blocks, rounded up: a block without keys costs more than it
+// gives (16 heads, in a graph, whole / cluster: 128 keys 6.0 / 5.9 us by 2, 6.4 by 8; 256 keys 7.6 / 6.2 by 4, 6.6 by 8;
+// 511 keys 10.6 / 6.6 by 8).
 static int cluster_size(const LbPagedAttnArgs& a) {
   const long long blocks = most_blocks(a);
-  if (a.cu_q || blocks <= NOSPLIT_BLOCKS) return 0;
+  if (a.cu_q || blocks <= 2) return 0;
   const int rows = eight_rows(a) ? 8 : 16;
   const long long items = (long long)a.n_seqs * a.Hkv * ((a.H / a.Hkv + rows - 1) / rows);
   for (int cl = 8; cl > 1; cl /= 2)
-    if (items * cl <= 2ll * num_sms() && blocks <= (long long)cl * FEW_BLOCKS) return cl;
+    if (cl < 2 * blocks && items * cl <= 2ll * num_sms() && blocks <= (long long)cl * FEW_BLOCKS) return cl;
   return 0;
 }
 template <int NT>
