@@ -13,7 +13,7 @@ namespace lb {
 // (8 channels, 4 rotation pairs) of a token and AP_HEADS of its heads, so that position, page and cos / sin row are found
 // once for all of them; the heads' loads are issued before that search (sequence, length, page: a chain of dependent reads)
 // and arrive while it runs. 24 prompts, 2532 tokens of 48
-// heads (64 MB): 10.7 us, 6.0 TB/s, in a graph (one head to a thread: 31 us a call, now 20 us, most of it the host's).
+// heads (64 MB): 10.7 us, 6.0 TB/s, in a graph (one head to a thread: 31 us a call, now 17 us, most of it the host's).
 constexpr int AP_HEADS = 8;
 __global__ void __launch_bounds__(128) paged_append_kernel(const LbPagedAppendArgs a) {
   const int vph = a.D / 8, v = threadIdx.x & (vph - 1);  // 8 or 16 vectors of a head
