@@ -28,7 +28,7 @@ def _knob(value: Knob, name: str, N: int, neutral: float, dev: int):
 def _rows(t: Optional[torch.Tensor], dtype: torch.dtype, shape, dev: int) -> bool:
     """An operand that is absent, or as the kernel reads it: rows of ``shape`` without gaps inside them."""
     return t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == dev
-                         and (shape[-1] <= 1 or t.stride(-1) == 1))
+                         and (t.is_contiguous() or shape[-1] <= 1 or t.stride(-1) == 1))
 
 
 def _torn(out: torch.Tensor, logits: torch.Tensor) -> bool:
@@ -40,8 +40,10 @@ def _torn(out: torch.Tensor, logits: torch.Tensor) -> bool:
     end = [t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + V) * es for t in (out, logits)]
     if a >= end[1] or b >= end[0]:
         return False
+    if out.shape[0] <= 1 or out.stride(0) != logits.stride(0):
+        return True
     row = out.stride(0) * es  # rows of one spacing may lie side by side
-    return out.stride(0) != logits.stride(0) or not V * es <= (a - b) % row <= row - V * es
+    return not V * es <= (a - b) % row <= row - V * es
 
 
 def penalize_logits_ref(logits, history, history_len, prompt_len=None, repetition=None, presence=None, frequency=None,
@@ -96,7 +98,8 @@ def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_len: to
             and _rows(history_len, i32, (N,), dev) and _rows(prompt_len, i32, (N,), dev)
             and (bias is None or _rows(bias, torch.float32, (V,) if bias.dim() == 1 else (N, V), dev))
             and _rows(allowed, i32, (N, (V + 31) // 32), dev)
-            and _rows(out, dt, (N, V), dev) and (out is None or ((N <= 1 or out.stride(0) >= V) and not _torn(out, logits))) and not _tracked(logits)):
+            and (out is None or (_rows(out, dt, (N, V), dev) and (N <= 1 or out.stride(0) >= V) and not _torn(out, logits)))
+            and not _tracked(logits)):
         # something is unusual: the reference path, or words for what is wrong
         _refuse(history.dim() != 2 or history.shape[0] != N or history.dtype != torch.int64, "history must be int64 [N, L]")
         for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):

@@ -150,3 +150,7 @@ def test_penalize_destinations():
     one = torch.zeros(1, 50)
     with pytest.raises(ValueError):
         L.penalize_logits(one[:, :40], hist[:1], hl[:1], out=one[:, 8:48])
+    flat = torch.zeros(60)
+    with pytest.raises(ValueError):
+        L.penalize_logits(flat[:40].expand(1, 40), hist[:1], hl[:1], out=flat[8:48].expand(1, 40))
+    L.penalize_logits(flat[:20].expand(1, 20), hist[:1], hl[:1], out=flat[20:40].expand(1, 20))
